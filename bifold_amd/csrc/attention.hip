@@ -413,7 +413,7 @@ __global__ __launch_bounds__(512) void attn_fwd_mfma_kernel(
             }
         };
         // p = exp2(s * sl2 - mref) in place (log2 domain; one FMA with the scale and the reference folded, one v_exp,
-        // one add per score, in packed pairs); returns this lane's partial row sum
+        // one add per score, in pairs); returns this lane's partial row sum
         auto probs = [&](f32x16 (&sacc)[2], float mref) -> float {
             f32x2 psum2 = {0.f, 0.f};
             const f32x2 sl2v = {sl2, sl2}, mneg = {-mref, -mref};
@@ -481,8 +481,8 @@ __global__ __launch_bounds__(512) void attn_fwd_mfma_kernel(
                 m = m_new;
             }
             const float m_use = (m == -INFINITY) ? 0.f : m;
-            // pairs of scores go through packed fp32 ops (v_pk_fma_f32 / v_pk_add_f32: two lanes' worth per
-            // instruction); the softmax, not the MFMA, bounds this kernel (28 VALU instructions per MFMA)
+            // scores are taken in pairs (two scalar instructions each: the Makefile switches packed fp32 off); the
+            // softmax, not the MFMA, bounds this kernel
             f32x2 psum2 = {0.f, 0.f};
             const f32x2 sl2v = {sl2, sl2}, mneg = {-m_use, -m_use};
 #pragma unroll
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(1024) void attn_fwd_res_kernel(
                 }
         }
     };
-    // p = exp2(s * sl2 - mref) IN PLACE; returns this lane's partial row sum (pairs of scores go through packed fp32 ops)
+    // p = exp2(s * sl2 - mref) IN PLACE; returns this lane's partial row sum (scores in pairs)
     auto probs = [&](f32x16 (&sacc)[NKB], float mref) -> float {
         f32x2 psum2 = {0.f, 0.f};
         const f32x2 sl2v = {sl2, sl2}, mneg = {-mref, -mref};
@@ -760,8 +760,8 @@ __global__ __launch_bounds__(1024) void attn_fwd_res_kernel(
                 m = m_new;
             }
             const float m_use = (m == -INFINITY) ? 0.f : m;
-            // pairs of scores go through packed fp32 ops (v_pk_fma_f32 / v_pk_add_f32: two lanes' worth per
-            // instruction); the softmax, not the MFMA, bounds this kernel (28 VALU instructions per MFMA)
+            // scores are taken in pairs (two scalar instructions each: the Makefile switches packed fp32 off); the
+            // softmax, not the MFMA, bounds this kernel
             f32x2 psum2 = {0.f, 0.f};
             const f32x2 sl2v = {sl2, sl2}, mneg = {-m_use, -m_use};
 #pragma unroll
@@ -1324,7 +1324,7 @@ __global__ __launch_bounds__(512) void attn_bwd_q_kernel(
         constexpr bool EDGE = decltype(edge_c)::value;
         const f32x2 sl2v = {sl2, sl2};
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {                   // packed fp32: two scores per VALU instruction
+        for (int e = 0; e < 16; e += 2) {                   // two scores at a time
             const f32x2 t = (f32x2){sacc[e], sacc[e + 1]} * sl2v;
             const f32x2 p2 = {__builtin_amdgcn_exp2f(t[0]), __builtin_amdgcn_exp2f(t[1])};
             const f32x2 ds2 = p2 * (f32x2){pacc[e], pacc[e + 1]};
@@ -1560,7 +1560,7 @@ __global__ __launch_bounds__(512, WPE) void attn_bwd_kv_kernel(
         // own lane's dK / dV columns, which are never stored) and the factor `scale` of dS (applied once, to dK at the end)
         const f32x2 sl2v = {sl2, sl2};
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {                   // packed fp32: two scores per VALU instruction
+        for (int e = 0; e < 16; e += 2) {                   // two scores at a time
             const f32x2 t = (f32x2){sacc[e], sacc[e + 1]} * sl2v;
             f32x2 p2 = {__builtin_amdgcn_exp2f(t[0]), __builtin_amdgcn_exp2f(t[1])};
             f32x2 ds2 = p2 * (f32x2){pacc[e], pacc[e + 1]};

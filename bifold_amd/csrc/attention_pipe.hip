@@ -767,7 +767,7 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_kv_pipe_kernel(
     };
     // p = exp2(S' c), dS = p dP', both packed for the products above
     auto v_phase = [&](const f32x16& sX, const f32x16& pX, x8 (&pp)[2], x8 (&ds)[2]) __attribute__((always_inline)) {
-        // the two multiplies per score as packed fp32 pairs (v_pk_mul_f32: two elements per issue slot; same products)
+        // the two multiplies per score in pairs (two scalar instructions: the Makefile switches packed fp32 off)
         const f32x2 sl22 = {sl2, sl2};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -1076,7 +1076,7 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_q_pipe_kernel(
             }
     };
     auto v_phase = [&](const f32x16& sX, const f32x16& pX, float cl, x8 (&ds)[2]) __attribute__((always_inline)) {
-        // the FMA of the exponent and the product with dP as packed fp32 pairs (v_pk_fma_f32 / v_pk_mul_f32: same values)
+        // the FMA of the exponent and the product with dP in pairs (as above)
         const f32x2 sl22 = {sl2, sl2}, cl2 = {cl, cl};
 #pragma unroll
         for (int u = 0; u < 2; ++u)

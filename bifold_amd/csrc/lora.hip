@@ -48,7 +48,7 @@ template <> __device__ __forceinline__ float4 half4_to_f32<f16_t>(uint2 w) {
     const f16x4 h = __builtin_bit_cast(f16x4, w);
     return make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
 }
-// four columns of a lane as two packed pairs (v_pk_fma_f32: two FMAs per issue slot)
+// four columns of a lane as two pairs (scalar FMAs: the Makefile switches packed fp32 off)
 struct Quad { f32x2 lo, hi; };
 __device__ __forceinline__ Quad quad_zero() { Quad q; q.lo = (f32x2){0.f, 0.f}; q.hi = (f32x2){0.f, 0.f}; return q; }
 __device__ __forceinline__ Quad quad_of(float4 v, float a) { Quad q; q.lo = (f32x2){v.x * a, v.y * a}; q.hi = (f32x2){v.z * a, v.w * a}; return q; }
