@@ -1,0 +1,151 @@
+// The 8-bit activation checkpoint (act8.hip, rmsnorm.hip): vector loads and stores of any alignment, the group's exponent,
+// the conversion both ways.
+//
+// A row is cut into groups of 32 columns, the last one possibly shorter.  A group shares one power of two, 2^e, with e the
+// smallest exponent for which round(max |x| 2^-e) <= 127 (and >= -126); element x is kept as q = round(x 2^-e), ties to
+// even, in int8, and reads back as q 2^e.  Powers of two make the scaling exact: the one rounding is q's, off by at most
+// 2^(e-1) <= max |x| / 127, and q 2^e is exact in fp32, bf16 and (inside its range) fp16.  The byte kept per group is
+// code = e + 127, the exponent field of 2^e as a float: 1 .. 247.  A group that holds a NaN, an infinity or a magnitude of
+// 255 * 2^119 or more gets code 255, q = 0: 2^e is then infinity as a float and every element reads back as NaN, so an
+// overflow still reaches the gradients (a loss scaler's check sees it).
+#pragma once
+#include "common.h"
+
+#define ACT8_GROUP 32
+
+// V consecutive elements as fp32.  AL: the address is aligned to the vector (at most 16 bytes); otherwise only to the element
+// -- global memory takes unaligned 16-byte accesses on this target, so an odd width costs split cache lines and no scalar path.
+template <typename T, int V, bool AL>
+__device__ __forceinline__ void vec_load(const T* p, float (&o)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec r;
+    constexpr int A = sizeof(vec) < 16 ? sizeof(vec) : 16;
+    if constexpr (AL) __builtin_memcpy(&r, __builtin_assume_aligned(p, A), sizeof(vec));
+    else __builtin_memcpy(&r, p, sizeof(vec));
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = to_f32<T>(r[j]);
+}
+template <typename T, int V, bool AL>
+__device__ __forceinline__ void vec_store(T* p, const float (&v)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r[j] = from_f32<T>(v[j]);
+    constexpr int A = sizeof(vec) < 16 ? sizeof(vec) : 16;
+    if constexpr (AL) __builtin_memcpy(__builtin_assume_aligned(p, A), &r, sizeof(vec));
+    else __builtin_memcpy(p, &r, sizeof(vec));
+}
+// the same with only n of the V elements there (n <= 0: none); the others read as zero and are not written.  With AL a
+// vector is there as a whole or not at all.
+template <typename T, int V, bool AL>
+__device__ __forceinline__ void vec_load_n(const T* p, int n, float (&o)[V]) {
+    if (n >= V) {
+        vec_load<T, V, AL>(p, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = !AL && j < n ? to_f32<T>(p[j]) : 0.f;
+    }
+}
+template <typename T, int V, bool AL>
+__device__ __forceinline__ void vec_store_n(T* p, int n, const float (&v)[V]) {
+    if (n >= V) {
+        vec_store<T, V, AL>(p, v);
+    } else if constexpr (!AL) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n) p[j] = from_f32<T>(v[j]);
+    }
+}
+// V bytes <-> V / 4 words
+template <int V, bool AL>
+__device__ __forceinline__ void bytes_store_n(uint8_t* p, int n, const unsigned (&w)[V / 4]) {
+    if (n >= V) {
+        if constexpr (AL) __builtin_memcpy(__builtin_assume_aligned(p, V), w, V);
+        else __builtin_memcpy(p, w, V);
+    } else if constexpr (!AL) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n) p[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+    }
+}
+template <int V, bool AL>
+__device__ __forceinline__ void bytes_load_n(const uint8_t* p, int n, unsigned (&w)[V / 4]) {
+    if (n >= V) {
+        if constexpr (AL) __builtin_memcpy(w, __builtin_assume_aligned(p, V), V);
+        else __builtin_memcpy(w, p, V);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) w[j] = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (!AL && j < n) w[j >> 2] |= (unsigned)p[j] << (8 * (j & 3));
+    }
+}
+
+// Largest magnitude of V elements as the bits of a non-negative float: an integer maximum, so a NaN (whose bits lie above
+// infinity's) is kept where fmaxf would drop it.
+template <int V>
+__device__ __forceinline__ unsigned magnitude_bits(const float (&x)[V]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const unsigned b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+        m = m > b ? m : b;
+    }
+    return m;
+}
+// maximum over the 32 / V neighbouring lanes that hold one group (V = 8: a quad, V = 4: two quads).  All lanes of the group
+// must be active.
+template <int V>
+__device__ __forceinline__ unsigned group_max(unsigned v) {
+    static_assert(V == 8 || V == 4, "a group is a quad of 8-element lanes or eight 4-element lanes");
+    unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);       // quad_perm [1, 0, 3, 2]
+    v = v > o ? v : o;
+    o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);                // quad_perm [2, 3, 0, 1]
+    v = v > o ? v : o;
+    if constexpr (V == 4) {
+        o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true);           // row_half_mirror: the other quad
+        v = v > o ? v : o;
+    }
+    return v;
+}
+
+// The group's byte.  With max |x| = m 2^k, 1 <= m < 2, e = k - 6 puts it into [64, 128); where it would round to 128
+// (m >= 255 / 128, mantissa field >= 0x7F0000) adding 0x10000 carries into the exponent field.
+__device__ __forceinline__ unsigned act8_code(unsigned amax_bits) {
+    const int c = (int)((amax_bits + 0x10000u) >> 23) - 6;
+    return c >= 248 ? 255u : c < 1 ? 1u : (unsigned)c;
+}
+__device__ __forceinline__ float act8_step(unsigned code) { return __uint_as_float(code << 23); }      // 2^e; 255: infinity
+
+// Four elements to four bytes: x 2^-e + 1.5 * 2^23 rounds to an integer (ties to even) whose two's complement is the low
+// byte of the sum's bits; two byte permutes join them.
+__device__ __forceinline__ unsigned act8_quant4(float a, float b, float c, float d, float inv) {
+    const float magic = 12582912.0f;
+    const unsigned ia = __float_as_uint(fmaf(a, inv, magic)), ib = __float_as_uint(fmaf(b, inv, magic));
+    const unsigned ic = __float_as_uint(fmaf(c, inv, magic)), id = __float_as_uint(fmaf(d, inv, magic));
+    const unsigned lo = __builtin_amdgcn_perm(ib, ia, 0x0c0c0400u), hi = __builtin_amdgcn_perm(id, ic, 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+template <int V>
+__device__ __forceinline__ void act8_quant(const float (&x)[V], unsigned code, unsigned (&w)[V / 4]) {
+    const float inv = __uint_as_float((254u - code) << 23);                              // 2^-e (not used for code 255)
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+        const unsigned q = act8_quant4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3], inv);
+        w[j] = code == 255u ? 0u : q;
+    }
+}
+// q 2^e = (u - 128) 2^e with u = q + 128 unsigned (one conversion instruction per byte); both terms and the sum are exact.
+template <int V>
+__device__ __forceinline__ void act8_dequant(const unsigned (&w)[V / 4], unsigned code, float (&x)[V]) {
+    const float s = act8_step(code), off = -128.0f * s;
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+        const unsigned u = w[j] ^ 0x80808080u;
+        x[4 * j] = fmaf((float)(u & 255u), s, off);
+        x[4 * j + 1] = fmaf((float)((u >> 8) & 255u), s, off);
+        x[4 * j + 2] = fmaf((float)((u >> 16) & 255u), s, off);
+        x[4 * j + 3] = fmaf((float)(u >> 24), s, off);
+    }
+}

@@ -1,0 +1,183 @@
+// Activation checkpoints in 8 bits (format: act8.h) and their use in the backward pass:
+//   bf_act8_pack       x -> q, code                       what a training step keeps instead of a 16- or 32-bit activation
+//   bf_act8_unpack     q, code -> x
+//   bf_act8_gelu_fwd   pre -> y = act(pre), and the checkpoint of pre, in one pass
+//   bf_act8_gelu_bwd   dy, checkpoint -> dpre = dy act'(q 2^e)
+// All four stream: every byte is touched once and nothing is reused, so HBM bounds them and the layout is chosen for it.  A
+// lane holds 8 consecutive elements (one 16-byte access of a 16-bit tensor, two of an fp32 one, 8 bytes of q); a group of 32
+// is a quad of lanes, its maximum two cross-lane moves without LDS.
+#include "act8.h"
+
+namespace {
+
+enum { A8_PACK = 0, A8_UNPACK = 1, A8_FWD = 2, A8_BWD = 3 };
+
+// ---- the activations.  s = 1 / (1 + e^-u):  quick GELU x s(1.702 x);  tanh GELU x s(2 c (x + 0.044715 x^3)), which is
+// 0.5 x (1 + tanh) without its cancellation at negative x;  erf GELU x Phi(x).  Derivative of x s(u): s + x u' s (1 - s).
+// fp32 tensors take the accurate exponential and division; 16-bit ones v_exp / v_rcp (relative error some 2^-21, the
+// result is rounded to 2^-9 or 2^-12).  |x| is cut at 100 in the derivative (in fp32 it is 0 or 1 from there on), a NaN stays.
+template <int ACT, bool EXACT> __device__ __forceinline__ float gate(float x) {
+    const float u = ACT == BF_ACT_QUICK_GELU ? 1.702f * x : 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
+    if constexpr (EXACT) return 1.0f / (1.0f + expf(-u));
+    else return __builtin_amdgcn_rcpf(1.0f + __expf(-u));
+}
+template <int ACT, bool EXACT> __device__ __forceinline__ float act_value(float x) {
+    if constexpr (ACT == BF_ACT_ERF_GELU) {
+        if constexpr (EXACT) return 0.5f * x * erfcf(-0.70710678118654752440f * x);
+        else return erf_gelu_fast(x);
+    } else {
+        return x * gate<ACT, EXACT>(x);
+    }
+}
+template <int ACT, bool EXACT> __device__ __forceinline__ float act_slope(float x) {
+    x = fabsf(x) > 100.0f ? copysignf(100.0f, x) : x;
+    if constexpr (ACT == BF_ACT_ERF_GELU) {
+        if constexpr (EXACT)
+            return 0.5f * erfcf(-0.70710678118654752440f * x) + x * 0.39894228040143267794f * expf(-0.5f * x * x);
+        else return erf_gelu_grad_fast(x);
+    } else {
+        const float s = gate<ACT, EXACT>(x);
+        const float du = ACT == BF_ACT_QUICK_GELU ? 1.702f : 1.5957691216057308f * fmaf(0.134145f * x, x, 1.0f);
+        // 1 - s as the gate of the other side where an fp32 result could show the cancellation
+        const float r = EXACT ? gate<ACT, EXACT>(-x) : 1.0f - s;
+        return fmaf(x * du, s * r, s);
+    }
+}
+
+// One kernel body for the four: MODE picks what is read and written.  DENSE: cols is a multiple of 32, all rows follow each
+// other and are 16-byte aligned, so vector v lies at element 8 v.  Otherwise a row owns a whole number of quads of lanes
+// (the last ones partly or wholly empty), `vpr` per row, and accesses may be unaligned: one division per 8 elements.
+struct A8Args {
+    const void* x; int64_t ldx;             // A8_PACK / A8_FWD: the activation;  A8_BWD: dy
+    void* y; int64_t ldy;                   // A8_FWD: act(pre);  A8_BWD: dpre;  A8_UNPACK: the tensor
+    uint8_t* q; uint8_t* code;
+    unsigned nvec; unsigned vpr; int cols; int gpr;
+};
+
+template <typename T, int MODE, int ACT, bool DENSE, int U>
+__global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
+    constexpr bool EXACT = sizeof(T) == 4;
+    const unsigned v0 = blockIdx.x * (256u * U) + threadIdx.x;
+    const T* x = (const T*)a.x;
+    T* y = (T*)a.y;
+    float f[U][8];
+    unsigned w[U][2], code[U];
+    size_t off_x[U], off_y[U], off_q[U], off_c[U];
+    int n[U];
+    bool first[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned v = v0 + u * 256u;
+        n[u] = v < a.nvec ? 8 : 0;
+        if constexpr (DENSE) {
+            off_x[u] = off_y[u] = off_q[u] = (size_t)v * 8;
+            off_c[u] = v >> 2;
+            first[u] = (v & 3) == 0 && n[u] > 0;
+        } else {
+            const unsigned row = v / a.vpr, c = (v - row * a.vpr) * 8;
+            if (n[u]) n[u] = min(8, a.cols - (int)c);          // <= 0 in the lanes that fill up the row's last group
+            off_x[u] = (size_t)row * a.ldx + c;
+            off_y[u] = (size_t)row * a.ldy + c;
+            off_q[u] = (size_t)row * a.cols + c;
+            off_c[u] = (size_t)row * a.gpr + (c >> 5);
+            first[u] = (c & 31) == 0 && n[u] > 0;
+        }
+        if constexpr (MODE == A8_UNPACK || MODE == A8_BWD) {
+            bytes_load_n<8, DENSE>(a.q + off_q[u], n[u], w[u]);
+            code[u] = n[u] > 0 ? a.code[off_c[u]] : 1u;
+        }
+        if constexpr (MODE != A8_UNPACK) vec_load_n<T, 8, DENSE>(x + off_x[u], n[u], f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if constexpr (MODE == A8_PACK || MODE == A8_FWD) {
+            code[u] = act8_code(group_max<8>(magnitude_bits<8>(f[u])));
+            act8_quant<8>(f[u], code[u], w[u]);
+            bytes_store_n<8, DENSE>(a.q + off_q[u], n[u], w[u]);
+            if (first[u]) a.code[off_c[u]] = (uint8_t)code[u];
+            if constexpr (MODE == A8_FWD) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[u][j] = act_value<ACT, EXACT>(f[u][j]);
+                vec_store_n<T, 8, DENSE>(y + off_y[u], n[u], f[u]);
+            }
+        } else {
+            float k[8];
+            act8_dequant<8>(w[u], code[u], k);
+            if constexpr (MODE == A8_BWD) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) k[j] = f[u][j] * act_slope<ACT, EXACT>(k[j]);
+            }
+            vec_store_n<T, 8, DENSE>(y + off_y[u], n[u], k);
+        }
+    }
+}
+
+template <typename T, int MODE, int ACT>
+void act8_launch(const A8Args& a, bool dense, hipStream_t s) {
+    // DENSE: four vectors per thread keep four (fp32: eight) 16-byte loads in flight per lane; two where addresses cost registers
+    if (dense) {
+        const unsigned blocks = (unsigned)(((size_t)a.nvec + 1023) / 1024);
+        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, true, 4>), dim3(blocks), dim3(256), 0, s, a);
+    } else {
+        const unsigned blocks = (unsigned)(((size_t)a.nvec + 511) / 512);
+        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, false, 2>), dim3(blocks), dim3(256), 0, s, a);
+    }
+}
+
+template <int MODE, int ACT>
+void act8_by_type(const A8Args& a, int dtype, bool dense, hipStream_t s) {
+    if (dtype == BF_BF16) act8_launch<bf16_t, MODE, ACT>(a, dense, s);
+    else if (dtype == BF_F16) act8_launch<f16_t, MODE, ACT>(a, dense, s);
+    else act8_launch<float, MODE, ACT>(a, dense, s);
+}
+
+template <int MODE>
+int act8_run(const char* name, const void* x, int64_t ldx, void* y, int64_t ldy, void* q, void* code, int dtype, int act,
+             int64_t rows, int cols, bf_stream_t stream) {
+    BF_REQUIRE(dtype == BF_F32 || bf_is_half(dtype), BF_EINVAL, "%s: bad dtype %d", name, dtype);
+    BF_REQUIRE(rows >= 0 && cols > 0, BF_EINVAL, "%s: bad shape (rows=%lld cols=%d)", name, (long long)rows, cols);
+    constexpr bool HAS_X = MODE != A8_UNPACK, HAS_Y = MODE != A8_PACK;
+    BF_REQUIRE((!HAS_X || ldx >= cols) && (!HAS_Y || ldy >= cols), BF_EINVAL, "%s: a leading dimension is under cols=%d", name, cols);
+    if (MODE == A8_FWD || MODE == A8_BWD)
+        BF_REQUIRE(act == BF_ACT_QUICK_GELU || act == BF_ACT_ERF_GELU || act == BF_ACT_TANH_GELU, BF_EINVAL,
+                   "%s: act must be BF_ACT_QUICK_GELU, BF_ACT_ERF_GELU or BF_ACT_TANH_GELU (got %d)", name, act);
+    if (rows == 0) return BF_OK;
+    BF_REQUIRE((!HAS_X || x) && (!HAS_Y || y) && q && code, BF_EINVAL, "%s: null pointer", name);
+    const size_t esz = bf_dtype_size(dtype);
+    BF_REQUIRE((!HAS_X || (uintptr_t)x % esz == 0) && (!HAS_Y || (uintptr_t)y % esz == 0), BF_EALIGN,
+               "%s: a tensor is not aligned to its element", name);
+    A8Args a;
+    a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy; a.q = (uint8_t*)q; a.code = (uint8_t*)code;
+    a.cols = cols; a.gpr = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
+    a.vpr = (unsigned)a.gpr * 4;
+    const unsigned long long nvec = (unsigned long long)rows * a.vpr;
+    BF_REQUIRE(nvec <= 0xFFFFF000ull, BF_EINVAL, "%s: rows=%lld x cols=%d is over 2^35 elements", name, (long long)rows, cols);
+    a.nvec = (unsigned)nvec;
+    const bool dense = cols % ACT8_GROUP == 0 && (!HAS_X || (ldx == cols && bf_aligned16(x))) &&
+                       (!HAS_Y || (ldy == cols && bf_aligned16(y))) && ((uintptr_t)q & 7u) == 0;
+    hipStream_t s = (hipStream_t)stream;
+    if (MODE == A8_PACK || MODE == A8_UNPACK) act8_by_type<MODE, BF_ACT_NONE>(a, dtype, dense, s);
+    else if (act == BF_ACT_QUICK_GELU) act8_by_type<MODE, MODE == A8_FWD || MODE == A8_BWD ? BF_ACT_QUICK_GELU : 0>(a, dtype, dense, s);
+    else if (act == BF_ACT_ERF_GELU) act8_by_type<MODE, MODE == A8_FWD || MODE == A8_BWD ? BF_ACT_ERF_GELU : 0>(a, dtype, dense, s);
+    else act8_by_type<MODE, MODE == A8_FWD || MODE == A8_BWD ? BF_ACT_TANH_GELU : 0>(a, dtype, dense, s);
+    BF_CHECK_LAUNCH(name);
+    return BF_OK;
+}
+
+}  // namespace
+
+extern "C" int bf_act8_pack(const void* x, int64_t ldx, int dtype, void* q, void* code, int64_t rows, int cols, bf_stream_t stream) {
+    return act8_run<A8_PACK>("bf_act8_pack", x, ldx, nullptr, 0, q, code, dtype, 0, rows, cols, stream);
+}
+extern "C" int bf_act8_unpack(const void* q, const void* code, void* x, int64_t ldx, int dtype, int64_t rows, int cols,
+                              bf_stream_t stream) {
+    return act8_run<A8_UNPACK>("bf_act8_unpack", nullptr, 0, x, ldx, (void*)q, (void*)code, dtype, 0, rows, cols, stream);
+}
+extern "C" int bf_act8_gelu_fwd(const void* pre, int64_t ld_pre, void* y, void* q, void* code, int dtype, int act, int64_t rows,
+                                int cols, bf_stream_t stream) {
+    return act8_run<A8_FWD>("bf_act8_gelu_fwd", pre, ld_pre, y, cols, q, code, dtype, act, rows, cols, stream);
+}
+extern "C" int bf_act8_gelu_bwd(const void* dy, int64_t ld_dy, const void* q, const void* code, void* dpre, int64_t ld_dpre,
+                                int dtype, int act, int64_t rows, int cols, bf_stream_t stream) {
+    return act8_run<A8_BWD>("bf_act8_gelu_bwd", dy, ld_dy, dpre, ld_dpre, (void*)q, (void*)code, dtype, act, rows, cols, stream);
+}

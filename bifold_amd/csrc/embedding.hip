@@ -1,0 +1,506 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//   bf_embed_scaled_fwd   out[i, :] = scale * table[id_i, :]
+//   bf_embed_scaled_bwd   grad[v, :] (+)= scale * sum over { i : id_i = v } of dy[i, :]
+// The gradient is a sum over rows that share a token.  Rows are brought together by a stable radix sort of (id, i), summed in
+// runs of equal ids in the order of i, each in fp32; nothing is added with atomics, so the result is the same on every call.
+// HBM bounds both for real batches (dy read once, the table's gradient written once); the sort's few kernels are short and
+// dependent, so the zeros of a dense gradient are written by further workgroups of the same launches.
+#include "act8.h"
+
+namespace {
+
+// ------------------------------------------------------------------ lookup
+template <typename TT, bool AL>
+__global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __restrict__ ids, const TT* __restrict__ table,
+                                                           void* __restrict__ out, int out_dtype, float scale, unsigned nvec,
+                                                           unsigned vpr, int cols, int vocab, int* __restrict__ err_flag) {
+    constexpr int V = sizeof(TT) == 4 ? 4 : 8, U = 4;
+    float f[U][V];
+    size_t off[U];
+    int n[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned v = blockIdx.x * (256u * U) + u * 256u + threadIdx.x;
+        const unsigned row = v / vpr, c = (v - row * vpr) * V;
+        n[u] = v < nvec ? cols - (int)c : 0;
+        off[u] = (size_t)row * cols + c;
+        int id = 0;
+        if (n[u] > 0) {
+            id = ids[row];
+            if (id < 0 || id >= vocab) {
+                if (c == 0 && err_flag) atomicExch(err_flag, 1);
+                id = 0;
+            }
+        }
+        vec_load_n<TT, V, AL>(table + (size_t)id * cols + c, n[u], f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[u][j] *= scale;
+        if (out_dtype == BF_F32) vec_store_n<float, V, AL>((float*)out + off[u], n[u], f[u]);
+        else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)out + off[u], n[u], f[u]);
+        else vec_store_n<f16_t, V, AL>((f16_t*)out + off[u], n[u], f[u]);
+    }
+}
+
+// ------------------------------------------------------------------ zeros of the dense gradient, in shares
+struct ZeroJob { float* p; size_t n; unsigned first, blocks; };            // workgroups [first, first + blocks) of the launch
+__device__ __forceinline__ void zero_share(const ZeroJob& z) {
+    const size_t at = (size_t)(blockIdx.x - z.first) * blockDim.x + threadIdx.x, step = (size_t)z.blocks * blockDim.x;
+    const size_t n4 = ((uintptr_t)z.p & 15u) == 0 ? z.n >> 2 : 0;
+    for (size_t i = at; i < n4; i += step) ((float4*)z.p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (size_t i = n4 * 4 + at; i < z.n; i += step) z.p[i] = 0.f;
+}
+__global__ __launch_bounds__(512) void embed_zero_kernel(const ZeroJob z) { zero_share(z); }
+
+// ------------------------------------------------------------------ the sort: least significant digit first, stable
+// A pass is two launches: counts of each digit per tile, then every tile finds its places -- for each digit the tokens of
+// smaller digits, of earlier tiles and of earlier waves -- and moves its tokens.  Digits of up to 9 bits put a vocabulary of
+// 2^18 into two passes.  Ids outside the table and the padding token become the key `vocab`, which sorts behind the others.
+#define SORT_THREADS 512
+#define SORT_WAVES 8
+#define SORT_MAX_BINS 512
+#define SORT_MAX_TILES 64
+
+struct SortArgs {
+    const int32_t* ids; int n; int vocab; int pad;
+    const int* keys_in; const int* idx_in; int* keys_out; int* idx_out;
+    int* hist; int* owner_count; int* err_flag;
+    int rounds, tiles, dbits, shift;
+    ZeroJob zero;
+};
+template <bool FIRST>
+__device__ __forceinline__ int sort_key(const SortArgs& a, int i, int* err_flag) {
+    if constexpr (FIRST) {
+        const int id = a.ids[i];
+        if (id < 0 || id >= a.vocab) {
+            if (err_flag) atomicExch(err_flag, 1);
+            return a.vocab;
+        }
+        return id == a.pad ? a.vocab : id;
+    } else {
+        return a.keys_in[i];
+    }
+}
+template <bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void embed_hist_kernel(const SortArgs a) {
+    __shared__ int bins[SORT_MAX_BINS];
+    if ((int)blockIdx.x >= a.tiles) { zero_share(a.zero); return; }
+    if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) *a.owner_count = 0;
+    bins[threadIdx.x] = 0;
+    __syncthreads();
+    const int span = SORT_THREADS * a.rounds, base = blockIdx.x * span, mask = (1 << a.dbits) - 1;
+    for (int r = 0; r < a.rounds; ++r) {
+        const int i = base + r * SORT_THREADS + threadIdx.x;
+        if (i < a.n) atomicAdd(&bins[(sort_key<FIRST>(a, i, a.err_flag) >> a.shift) & mask], 1);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x <= mask) a.hist[blockIdx.x * SORT_MAX_BINS + threadIdx.x] = bins[threadIdx.x];
+}
+template <bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortArgs a) {
+    __shared__ int cnt[SORT_WAVES][SORT_MAX_BINS];
+    __shared__ int wave_tot[SORT_WAVES];
+    if ((int)blockIdx.x >= a.tiles) { zero_share(a.zero); return; }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int mask = (1 << a.dbits) - 1;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) cnt[w][tid] = 0;
+    // all tokens of this digit, and those in earlier tiles
+    int tot = 0, before = 0;
+    if (tid <= mask) {
+#pragma unroll 8
+        for (int t = 0; t < a.tiles; ++t) {
+            const int h = a.hist[t * SORT_MAX_BINS + tid];
+            tot += h;
+            before += t < (int)blockIdx.x ? h : 0;
+        }
+    }
+    int scan = tot;                             // inclusive over the digits
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(scan, o, 64);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 63) wave_tot[wave] = scan;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) scan += wave_tot[w];
+    int place = scan - tot + before;
+    // a wave owns `rounds` x 64 consecutive tokens of the tile
+    const int first = blockIdx.x * SORT_THREADS * a.rounds + wave * 64 * a.rounds + lane;
+    for (int r = 0; r < a.rounds; ++r) {
+        const int i = first + r * 64;
+        if (i < a.n) atomicAdd(&cnt[wave][(sort_key<FIRST>(a, i, nullptr) >> a.shift) & mask], 1);
+    }
+    __syncthreads();
+    for (int w = 0; w < SORT_WAVES; ++w) {
+        const int c = cnt[w][tid];
+        cnt[w][tid] = place;
+        place += c;
+    }
+    __syncthreads();
+    // cnt[wave][d] is where this wave's next token of digit d goes.  Within 64 tokens the lanes of one digit find each other
+    // by a ballot per digit bit; the first of them moves the place on.  LDS accesses of one wave complete in order; the
+    // relaxed atomics keep the compiler from holding a place in a register.
+    int* mine = cnt[wave];
+    for (int r = 0; r < a.rounds; ++r) {
+        const int i = first + r * 64;
+        const bool live = i < a.n;
+        const int key = live ? sort_key<FIRST>(a, i, nullptr) : 0, d = (key >> a.shift) & mask;
+        unsigned long long same = __ballot(live);
+        for (int b = 0; b < a.dbits; ++b) {
+            const bool bit = (d >> b) & 1;
+            const unsigned long long votes = __ballot(bit);
+            same &= bit ? votes : ~votes;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1ull));
+        if (live) {
+            const int at = __hip_atomic_load(&mine[d], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            a.keys_out[at + rank] = key;
+            a.idx_out[at + rank] = FIRST ? i : a.idx_in[i];
+            if (rank == 0) __hip_atomic_store(&mine[d], at + __popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ sums over runs of equal keys
+struct SumArgs {
+    const int* keys; const int* idx; int n; int vocab; int chunk, chunks, slabs;
+    const void* dy; int64_t ld; int cols; float scale; int accumulate;
+    float* grad; float* part; int* owners; int* owner_count;
+};
+template <int V, bool AL>
+__device__ __forceinline__ void grad_write(const SumArgs& a, int key, int c, const float (&acc)[V]) {
+    float* g = a.grad + (size_t)key * a.cols + c;
+    float o[V];
+    if (a.accumulate) vec_load_n<float, V, AL>(g, a.cols - c, o);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = a.accumulate ? o[j] + acc[j] * a.scale : acc[j] * a.scale;
+    vec_store_n<float, V, AL>(g, a.cols - c, o);
+}
+// One wave takes `chunk` (at most 64) consecutive sorted tokens and 64 V columns, eight rows in flight.  A run that lies
+// inside the chunk goes to the gradient; the sum of a run that reaches over an end goes to part[chunk][0] (it began in an
+// earlier chunk) or part[chunk][1] (it begins here: this chunk owns the run and is noted for embed_join_kernel).
+template <typename T, int V, bool AL>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
+    const int lane = threadIdx.x & 63;
+    const unsigned w = blockIdx.x * 4u + (threadIdx.x >> 6);
+    const int chunk = (int)(w / (unsigned)a.slabs), slab = (int)(w - (unsigned)chunk * (unsigned)a.slabs);
+    if (chunk >= a.chunks) return;
+    const int s = chunk * a.chunk, here = min(a.chunk, a.n - s);
+    const int kl = lane < here ? a.keys[s + lane] : a.vocab;
+    const int il = lane < here ? a.idx[s + lane] : 0;
+    const int prev = s > 0 ? a.keys[s - 1] : -1, next = s + here < a.n ? a.keys[s + here] : -1;
+    const int live = __popcll(__ballot(lane < here && kl < a.vocab));      // sorted: the live ones come first
+    const int c = (slab * 64 + lane) * V, nc = a.cols - c;
+    const T* dy = (const T*)a.dy + c;
+    float* part = a.part + (size_t)chunk * 2 * a.cols + c;
+    float acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+    bool head = live > 0 && __builtin_amdgcn_readlane(kl, 0) == prev;
+    for (int i0 = 0; i0 < live; i0 += 8) {
+        float f[8][V];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (i0 + u < live) {
+                const int row = __builtin_amdgcn_readlane(il, i0 + u);
+                vec_load_n<T, V, AL>(dy + (size_t)row * a.ld, nc, f[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = i0 + u;
+            if (i < live) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[j] += f[u][j];
+                const int key = __builtin_amdgcn_readlane(kl, i);
+                const bool last = i + 1 == here;
+                const int after = last ? next : __builtin_amdgcn_readlane(kl, i + 1);
+                if (after != key) {
+                    if (head) vec_store_n<float, V, AL>(part, nc, acc);
+                    else grad_write<V, AL>(a, key, c, acc);
+                    head = false;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+                } else if (last) {
+                    vec_store_n<float, V, AL>(head ? part : part + a.cols, nc, acc);
+                    if (!head && slab == 0 && lane == 0) a.owners[atomicAdd(a.owner_count, 1)] = chunk;
+                }
+            }
+        }
+    }
+}
+// One workgroup per owned run (their order in the list does not matter: each has a gradient row of its own) and 256 columns:
+// finds the last chunk that starts with the run's key, sums the partial rows in order, sixteen waves a share each.
+__global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
+    __shared__ float4 red[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int slabs = (a.cols + 255) / 256;
+    const int total = *a.owner_count * slabs;
+    for (int wk = blockIdx.x; wk < total; wk += gridDim.x) {
+        const int chunk = a.owners[wk / slabs], c = (wk % slabs) * 256 + lane * 4, nc = a.cols - c;
+        const int key = a.keys[(size_t)(chunk + 1) * a.chunk - 1];
+        int lo = chunk + 1, hi = a.chunks;      // chunk lo starts with the key; hi does not (or is behind the last)
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
+            const bool in = at < hi && a.keys[(size_t)at * a.chunk] == key;
+            lo += step * __popcll(__ballot(in));
+            hi = min(hi, lo + step);
+        }
+        const int many = lo - chunk + 1, share = (many + 15) >> 4;          // partial rows: part[chunk][1], part[chunk + 1 ..][0]
+        const int from = wave * share, to = min(many, from + share);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int t = from; t < to; ++t) {
+            float f[4];
+            vec_load_n<float, 4, false>(a.part + ((size_t)(chunk + t) * 2 + (t == 0)) * a.cols + c, nc, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] += f[j];
+        }
+        red[wave][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int k = 1; k < 16; ++k) {
+                const float4 f = red[k][lane];
+                acc[0] += f.x; acc[1] += f.y; acc[2] += f.z; acc[3] += f.w;
+            }
+            grad_write<4, false>(a, key, c, acc);
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------ few tokens: one launch, no sort
+// A workgroup per token: the first token of its id gathers the others' places in order and sums their rows, each wave 64 V
+// columns and a share of the rows.
+#define FEW 512
+template <typename T, int V, bool AL>
+__global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restrict__ ids, int pad, int* __restrict__ err_flag,
+                                                        const SumArgs a) {
+    __shared__ unsigned long long words[FEW / 64];
+    __shared__ unsigned short list[FEW];
+    __shared__ float red[FEW / 64][64 * V];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, me = blockIdx.x;
+    const int key = ids[me];
+    if (key < 0 || key >= a.vocab) {
+        if (tid == 0 && err_flag) atomicExch(err_flag, 1);
+        return;
+    }
+    if (key == pad) return;
+    const bool same = tid < a.n && ids[tid] == key;
+    const unsigned long long votes = __ballot(same);
+    if (lane == 0) words[wave] = votes;
+    __syncthreads();
+    int rank = __popcll(votes & ((1ull << lane) - 1ull)), many = 0;
+    bool earlier = false;
+#pragma unroll
+    for (int w = 0; w < FEW / 64; ++w) {
+        const unsigned long long v = words[w];
+        if (w < wave) rank += __popcll(v);
+        many += __popcll(v);
+        const int below = me - w * 64;          // tokens of this word in front of this one
+        earlier |= below >= 64 ? v != 0 : below > 0 ? (v & ((1ull << below) - 1ull)) != 0 : false;
+    }
+    if (earlier) return;                        // uniform: the first token of this id does the work
+    if (same) list[rank] = (unsigned short)tid;
+    __syncthreads();
+    const int waves = FEW / 64;
+    const int shares = a.slabs >= waves ? 1 : waves / a.slabs;
+    for (int slab0 = 0; slab0 < a.slabs; slab0 += waves) {
+        const int at = wave / shares, slab = slab0 + at, sh = wave - at * shares;
+        const bool in = slab < a.slabs && at < waves / shares;
+        const int per = (many + shares - 1) / shares, from = sh * per, to = in ? min(many, from + per) : 0;
+        const int c = (slab * 64 + lane) * V, nc = a.cols - c;
+        float acc[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll 4
+        for (int t = from; t < to; ++t) {
+            float f[V];
+            vec_load_n<T, V, AL>((const T*)a.dy + (size_t)list[t] * a.ld + c, nc, f);
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += f[j];
+        }
+        if (shares > 1) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) red[wave][j * 64 + lane] = acc[j];
+            __syncthreads();
+            if (sh == 0 && in) {
+                for (int k = 1; k < shares; ++k)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[j] += red[wave + k][j * 64 + lane];
+            }
+            __syncthreads();
+        }
+        if (sh == 0 && in) grad_write<V, AL>(a, key, c, acc);
+    }
+}
+
+// ------------------------------------------------------------------ plan of a call
+struct EmbedPlan {
+    int passes, dbits, rounds, tiles, chunk, chunks;
+    size_t keys, hist, owners, part, bytes;     // offsets into the workspace
+};
+EmbedPlan embed_plan(int n, int cols, int vocab) {
+    EmbedPlan p;
+    int bits = 0;
+    while (bits < 31 && (vocab >> bits) != 0) ++bits;            // the key `vocab` itself is used
+    p.passes = (bits + 8) / 9;
+    p.dbits = (bits + p.passes - 1) / p.passes;
+    const long span = (long)SORT_THREADS * SORT_MAX_TILES;
+    p.rounds = (int)((n + span - 1) / span);
+    p.tiles = (n + SORT_THREADS * p.rounds - 1) / (SORT_THREADS * p.rounds);
+    // tokens per wave: enough waves for the chip first, then few partial rows
+    p.chunk = n >= 65536 ? 64 : n >= 16384 ? 32 : 16;
+    p.chunks = (n + p.chunk - 1) / p.chunk;
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    p.keys = 0;
+    p.hist = up((size_t)n * 16);
+    p.owners = p.hist + up((size_t)p.tiles * SORT_MAX_BINS * 4);
+    p.part = p.owners + up((size_t)(p.chunks + 1) * 4);
+    p.bytes = p.part + up((size_t)p.chunks * 2 * cols * 4);
+    return p;
+}
+
+template <typename T, int V, bool AL>
+void embed_sum_launch(const SumArgs& a, hipStream_t s) {
+    const size_t waves = (size_t)a.chunks * a.slabs;
+    hipLaunchKernelGGL((embed_sum_kernel<T, V, AL>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+}
+template <typename T, int V>
+void embed_bwd_type(bool few, bool al, const int32_t* ids, int pad, int* err_flag, const SumArgs& a, hipStream_t s) {
+    if (few) {
+        if (al) hipLaunchKernelGGL((embed_few_kernel<T, V, true>), dim3((unsigned)a.n), dim3(FEW), 0, s, ids, pad, err_flag, a);
+        else hipLaunchKernelGGL((embed_few_kernel<T, V, false>), dim3((unsigned)a.n), dim3(FEW), 0, s, ids, pad, err_flag, a);
+    } else if (al) {
+        embed_sum_launch<T, V, true>(a, s);
+    } else {
+        embed_sum_launch<T, V, false>(a, s);
+    }
+}
+bool float_type(int dt) { return dt == BF_F32 || bf_is_half(dt); }
+
+}  // namespace
+
+extern "C" int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int table_dtype, void* out, int out_dtype, float scale,
+                                   int n, int cols, int vocab, int* err_flag, bf_stream_t stream) {
+    const char* name = "bf_embed_scaled_fwd";
+    BF_REQUIRE(float_type(table_dtype) && float_type(out_dtype), BF_EINVAL, "%s: bad table_dtype %d or out_dtype %d", name,
+               table_dtype, out_dtype);
+    BF_REQUIRE(n >= 0 && cols > 0 && vocab > 0, BF_EINVAL, "%s: bad shape (n=%d cols=%d vocab=%d)", name, n, cols, vocab);
+    if (n == 0) return BF_OK;
+    BF_REQUIRE(tokens && table && out, BF_EINVAL, "%s: null pointer", name);
+    const size_t ts = bf_dtype_size(table_dtype), os = bf_dtype_size(out_dtype);
+    BF_REQUIRE((uintptr_t)tokens % 4 == 0 && (uintptr_t)table % ts == 0 && (uintptr_t)out % os == 0, BF_EALIGN,
+               "%s: a tensor is not aligned to its element", name);
+    const int V = table_dtype == BF_F32 ? 4 : 8;
+    const unsigned vpr = (unsigned)((cols + V - 1) / V);
+    const unsigned long long nvec = (unsigned long long)n * vpr;
+    BF_REQUIRE(nvec <= 0xFFFFF000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
+    const bool al = cols % V == 0 && bf_aligned16(table) && bf_aligned16(out);
+    const dim3 grid((unsigned)((nvec + 1023) / 1024)), block(256);
+    hipStream_t s = (hipStream_t)stream;
+#define EMBED_FWD(T)                                                                                                             \
+    do {                                                                                                                         \
+        if (al) hipLaunchKernelGGL((embed_scaled_kernel<T, true>), grid, block, 0, s, tokens, (const T*)table, out, out_dtype,   \
+                                   scale, (unsigned)nvec, vpr, cols, vocab, err_flag);                                           \
+        else hipLaunchKernelGGL((embed_scaled_kernel<T, false>), grid, block, 0, s, tokens, (const T*)table, out, out_dtype,     \
+                                scale, (unsigned)nvec, vpr, cols, vocab, err_flag);                                              \
+    } while (0)
+    if (table_dtype == BF_F32) EMBED_FWD(float);
+    else if (table_dtype == BF_BF16) EMBED_FWD(bf16_t);
+    else EMBED_FWD(f16_t);
+#undef EMBED_FWD
+    BF_CHECK_LAUNCH(name);
+    return BF_OK;
+}
+
+extern "C" size_t bf_embed_scaled_bwd_workspace_bytes(int n, int cols, int vocab) {
+    if (n <= FEW || cols <= 0 || vocab <= 0) return 0;
+    return embed_plan(n, cols, vocab).bytes;
+}
+
+extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const int32_t* tokens, float* grad, float scale,
+                                   int accumulate, int padding_idx, int n, int cols, int vocab, int* err_flag, void* workspace,
+                                   size_t workspace_bytes, bf_stream_t stream) {
+    const char* name = "bf_embed_scaled_bwd";
+    BF_REQUIRE(float_type(dy_dtype), BF_EINVAL, "%s: bad dy_dtype %d", name, dy_dtype);
+    BF_REQUIRE(n >= 0 && cols > 0 && vocab > 0 && vocab < 0x7FFFFFFF, BF_EINVAL, "%s: bad shape (n=%d cols=%d vocab=%d)", name, n,
+               cols, vocab);
+    BF_REQUIRE(n <= (1 << 30), BF_EINVAL, "%s: over 2^30 tokens (n=%d)", name, n);
+    BF_REQUIRE(grad && (uintptr_t)grad % 4 == 0, BF_EALIGN, "%s: grad is null or not aligned to its element", name);
+    hipStream_t s = (hipStream_t)stream;
+    const size_t floats = accumulate ? 0 : (size_t)vocab * cols;
+    auto zero_job = [&](size_t from, size_t to, unsigned first) {
+        ZeroJob z = {grad + from, to - from, first, 0};
+        size_t b = (z.n + 8191) / 8192;                          // four 16-byte stores per thread, more for large tables
+        z.blocks = (unsigned)(b < 2048 ? b : 2048);
+        return z;
+    };
+    if (n <= FEW) {
+        const ZeroJob z = zero_job(0, floats, 0);
+        if (z.blocks) {
+            hipLaunchKernelGGL(embed_zero_kernel, dim3(z.blocks), dim3(512), 0, s, z);
+            BF_CHECK_LAUNCH(name);
+        }
+        if (n == 0) return BF_OK;
+    }
+    BF_REQUIRE(dy && tokens, BF_EINVAL, "%s: null pointer", name);
+    BF_REQUIRE(ld_dy >= cols, BF_EINVAL, "%s: ld_dy=%lld is under cols=%d", name, (long long)ld_dy, cols);
+    const size_t esz = bf_dtype_size(dy_dtype);
+    BF_REQUIRE((uintptr_t)dy % esz == 0 && (uintptr_t)tokens % 4 == 0, BF_EALIGN, "%s: a tensor is not aligned to its element", name);
+    const int V = dy_dtype == BF_F32 ? 4 : 8;
+    const bool al = cols % V == 0 && bf_aligned16(dy) && ((size_t)ld_dy * esz) % 16 == 0 && bf_aligned16(grad);
+    SumArgs a = {};
+    a.n = n; a.vocab = vocab; a.dy = dy; a.ld = ld_dy; a.cols = cols; a.scale = scale; a.accumulate = accumulate; a.grad = grad;
+    a.slabs = (cols + 64 * V - 1) / (64 * V);
+    const bool few = n <= FEW;
+    BF_REQUIRE((unsigned long long)n * a.slabs <= 0xFFFF0000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
+    if (!few) {
+        const EmbedPlan p = embed_plan(n, cols, vocab);
+        BF_REQUIRE(workspace && workspace_bytes >= p.bytes, BF_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", name,
+                   workspace_bytes, p.bytes);
+        BF_REQUIRE(bf_aligned16(workspace), BF_EALIGN, "%s: unaligned workspace", name);
+        char* ws = (char*)workspace;
+        int* buf[4];
+        for (int k = 0; k < 4; ++k) buf[k] = (int*)(ws + p.keys) + (size_t)k * n;
+        int* owners = (int*)(ws + p.owners);
+        SortArgs q = {};
+        q.ids = tokens; q.n = n; q.vocab = vocab; q.pad = padding_idx; q.hist = (int*)(ws + p.hist);
+        q.owner_count = owners + p.chunks; q.err_flag = err_flag; q.rounds = p.rounds; q.tiles = p.tiles; q.dbits = p.dbits;
+        const int launches = 2 * p.passes;
+        size_t done = 0;
+        for (int pass = 0; pass < p.passes; ++pass) {
+            q.shift = pass * p.dbits;
+            q.keys_in = buf[2 * ((pass + 1) & 1)]; q.idx_in = buf[2 * ((pass + 1) & 1) + 1];
+            q.keys_out = buf[2 * (pass & 1)]; q.idx_out = buf[2 * (pass & 1) + 1];
+            for (int half = 0; half < 2; ++half) {
+                const int k = 2 * pass + half + 1;
+                const size_t to = k == launches ? floats : floats / launches * k & ~(size_t)3;
+                q.zero = zero_job(done, to, (unsigned)p.tiles);
+                done = to;
+                const dim3 grid((unsigned)p.tiles + q.zero.blocks), block(SORT_THREADS);
+                if (half == 0 && pass == 0) hipLaunchKernelGGL((embed_hist_kernel<true>), grid, block, 0, s, q);
+                else if (half == 0) hipLaunchKernelGGL((embed_hist_kernel<false>), grid, block, 0, s, q);
+                else if (pass == 0) hipLaunchKernelGGL((embed_scatter_kernel<true>), grid, block, 0, s, q);
+                else hipLaunchKernelGGL((embed_scatter_kernel<false>), grid, block, 0, s, q);
+                BF_CHECK_LAUNCH(name);
+            }
+        }
+        a.keys = q.keys_out; a.idx = q.idx_out; a.chunk = p.chunk; a.chunks = p.chunks;
+        a.part = (float*)(ws + p.part); a.owners = owners; a.owner_count = owners + p.chunks;
+    }
+    if (dy_dtype == BF_F32) embed_bwd_type<float, 4>(few, al, tokens, padding_idx, err_flag, a, s);
+    else if (dy_dtype == BF_BF16) embed_bwd_type<bf16_t, 8>(few, al, tokens, padding_idx, err_flag, a, s);
+    else embed_bwd_type<f16_t, 8>(few, al, tokens, padding_idx, err_flag, a, s);
+    BF_CHECK_LAUNCH(name);
+    if (!few) {
+        const size_t most = (size_t)a.chunks * ((cols + 255) / 256);
+        hipLaunchKernelGGL(embed_join_kernel, dim3((unsigned)(most < 512 ? most : 512)), dim3(1024), 0, s, a);
+        BF_CHECK_LAUNCH(name);
+    }
+    return BF_OK;
+}

@@ -1,0 +1,594 @@
+// Root-mean-square norm with the residual's addition (forward, to 16 / 32 bits or to e4m3 with a row scale) and its backward.
+//   forward:   t = x + delta;  r = 1 / sqrt(mean t^2 + eps);  y = t r gamma
+//              e4m3: s = max |y| / 448 (1 for a row of zeros, NaN for one that holds a NaN or an infinity), y8 = e4m3(y / s)
+//   backward:  h = t r;  b = dy gamma;  dx = dres + r (b - h mean(b h));  dgamma = sum over rows of dy h
+// The forward can leave the 8-bit checkpoint of t (act8.h) from the registers that hold the row; the backward takes t as a
+// tensor or as that checkpoint.  Statistics and sums are fp32.  t enters y, r and the checkpoint unrounded; x_out is t
+// rounded once to the stream's type.
+//
+// HBM bounds both: each tensor is read once and written once, the row stays in registers between the sum and the output.  A
+// lane holds V consecutive elements per chunk: 4 of an fp32 stream, 8 of a 16-bit one (16 bytes either way).  Rows up to
+// 1 024 columns belong to one wave (reductions without LDS or barriers, four rows per workgroup); up to 8 192 to one
+// workgroup; longer ones are walked two or three times.
+#include "act8.h"
+
+namespace {
+
+enum { Y_E4M3 = 3 };                            // beside BF_F32 / BF_BF16 / BF_F16 as a store format
+#define RMS_FP8_MAX 448.0f
+
+struct RmsFwd {
+    const void* x; int64_t ldx;
+    const void* delta; int64_t ldd; int d_dtype;
+    const float* gamma;
+    void* x_out; int64_t ldo;
+    void* y; int y_dtype; float* y_scale; float* rstd;
+    uint8_t* q; uint8_t* code;
+    int rows, cols, gpr; float eps;
+};
+struct RmsBwd {
+    const void* dy; int64_t ldy;
+    const void* x; int64_t ldx; int x_dtype; const uint8_t* q; const uint8_t* code;
+    const float* gamma; const float* rstd;
+    const void* dres; int64_t ldr;
+    void* dx; int dx_dtype;
+    float* part;
+    int rows, cols, gpr, nblk;
+};
+
+template <int V, bool AL> __device__ __forceinline__ void load_as(const void* p, int dtype, size_t off, int n, float (&o)[V]) {
+    if (dtype == BF_F32) vec_load_n<float, V, AL>((const float*)p + off, n, o);
+    else if (dtype == BF_BF16) vec_load_n<bf16_t, V, AL>((const bf16_t*)p + off, n, o);
+    else vec_load_n<f16_t, V, AL>((const f16_t*)p + off, n, o);
+}
+template <int V, bool AL> __device__ __forceinline__ void store_as(void* p, int dtype, size_t off, int n, const float (&v)[V]) {
+    if (dtype == BF_F32) vec_store_n<float, V, AL>((float*)p + off, n, v);
+    else if (dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)p + off, n, v);
+    else vec_store_n<f16_t, V, AL>((f16_t*)p + off, n, v);
+}
+template <int V> __device__ __forceinline__ void to_e4m3(const float (&y)[V], float inv, unsigned (&w)[V / 4]) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+        float f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = fminf(RMS_FP8_MAX, fmaxf(-RMS_FP8_MAX, y[4 * j + k] * inv));
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+        w[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], p, true);
+    }
+}
+// a row's scale from the bits of its largest magnitude (infinity and NaN lie at 0x7F800000 and above)
+__device__ __forceinline__ float e4m3_scale(unsigned amax_bits) {
+    if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    return amax_bits ? fmaxf(__uint_as_float(amax_bits) / RMS_FP8_MAX, 1.17549435e-38f) : 1.0f;    // 1 / s stays finite
+}
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const unsigned w = (unsigned)__shfl_xor((int)v, o, 64);
+        v = v > w ? v : w;
+    }
+    return v;
+}
+// sum / maximum over the WPR waves that share a row; `red` has one slot per wave and is used once between barriers
+template <int WPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+    v = wave_sum(v);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) v += red[w];
+    }
+    return v;
+}
+template <int WPR> __device__ __forceinline__ unsigned row_max(unsigned v, unsigned* red) {
+    v = wave_max_bits(v);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) v = v > red[w] ? v : red[w];
+    }
+    return v;
+}
+template <int V, bool AL>
+__device__ __forceinline__ void keep8(const RmsFwd& a, int row, int c, int n, const float (&t)[V]) {
+    const unsigned code = act8_code(group_max<V>(magnitude_bits<V>(t)));
+    unsigned w[V / 4];
+    act8_quant<V>(t, code, w);
+    bytes_store_n<V, AL>(a.q + (size_t)row * a.cols + c, n, w);
+    if ((c & 31) == 0 && n > 0) a.code[(size_t)row * a.gpr + (c >> 5)] = (uint8_t)code;
+}
+
+// ------------------------------------------------------------------ forward, the row in registers (cols <= 64 WPR V NV)
+template <typename TX, int V, int WPR, int NV, bool AL>
+__global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
+    constexpr int T = 64 * WPR;
+    __shared__ float red_s[4];
+    __shared__ unsigned red_m[4];
+    const int row = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= a.rows) return;
+    const int slot = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const TX* x = (const TX*)a.x + (size_t)row * a.ldx;
+    float t[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * T + slot) * V;
+        vec_load_n<TX, V, AL>(x + c, a.cols - c, t[i]);
+    }
+    if (a.delta) {
+        float d[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            load_as<V, AL>(a.delta, a.d_dtype, (size_t)row * a.ldd + c, a.cols - c, d[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) t[i][j] += d[i][j];
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) s = fmaf(t[i][j], t[i][j], s);
+    if (a.x_out) {
+        TX* o = (TX*)a.x_out + (size_t)row * a.ldo;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            vec_store_n<TX, V, AL>(o + c, a.cols - c, t[i]);
+        }
+    }
+    if (a.q) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            keep8<V, AL>(a, row, c, a.cols - c, t[i]);
+        }
+    }
+    const float r = 1.0f / sqrtf(row_sum<WPR>(s, red_s) / (float)a.cols + a.eps);
+    if (a.rstd && slot == 0) a.rstd[row] = r;
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * T + slot) * V;
+        float g[V];
+        vec_load_n<float, V, AL>(a.gamma + c, a.cols - c, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[i][j] = t[i][j] * r * g[j];
+        const unsigned b = magnitude_bits<V>(t[i]);
+        m = m > b ? m : b;
+    }
+    const size_t yo = (size_t)row * a.cols;
+    if (a.y_dtype == Y_E4M3) {
+        const float sc = e4m3_scale(row_max<WPR>(m, red_m)), inv = 1.0f / sc;
+        if (slot == 0) a.y_scale[row] = sc;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            unsigned w[V / 4];
+            to_e4m3<V>(t[i], inv, w);
+            bytes_store_n<V, AL>((uint8_t*)a.y + yo + c, a.cols - c, w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            store_as<V, AL>(a.y, a.y_dtype, yo + c, a.cols - c, t[i]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ forward, any width: one workgroup walks the row
+template <typename TX>
+__global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
+    constexpr int V = 8;
+    __shared__ float red_s[4];
+    __shared__ unsigned red_m[4];
+    const int row = blockIdx.x;
+    const TX* x = (const TX*)a.x + (size_t)row * a.ldx;
+    // t of this thread's chunk; x is read before x_out (which may be x) is written, and only by this thread
+    auto chunk = [&](int c, float (&t)[V]) __attribute__((always_inline)) {
+        vec_load_n<TX, V, false>(x + c, a.cols - c, t);
+        if (a.delta) {
+            float d[V];
+            load_as<V, false>(a.delta, a.d_dtype, (size_t)row * a.ldd + c, a.cols - c, d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) t[j] += d[j];
+        }
+    };
+    auto scaled = [&](int c, float r, float (&t)[V]) __attribute__((always_inline)) {
+        float g[V];
+        vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = t[j] * r * g[j];
+    };
+    float t[V], s = 0.f;
+    for (int base = 0; base < a.cols; base += 256 * V) {
+        const int c = base + threadIdx.x * V;
+        chunk(c, t);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s = fmaf(t[j], t[j], s);
+        if (a.q) keep8<V, false>(a, row, c, a.cols - c, t);
+    }
+    const float r = 1.0f / sqrtf(row_sum<4>(s, red_s) / (float)a.cols + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = r;
+    float inv = 1.0f;
+    if (a.y_dtype == Y_E4M3) {
+        unsigned m = 0;
+        for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
+            chunk(c, t);
+            scaled(c, r, t);
+            const unsigned b = magnitude_bits<V>(t);
+            m = m > b ? m : b;
+        }
+        const float sc = e4m3_scale(row_max<4>(m, red_m));
+        if (threadIdx.x == 0) a.y_scale[row] = sc;
+        inv = 1.0f / sc;
+    }
+    const size_t yo = (size_t)row * a.cols;
+    for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
+        chunk(c, t);
+        if (a.x_out) vec_store_n<TX, V, false>((TX*)a.x_out + (size_t)row * a.ldo + c, a.cols - c, t);
+        scaled(c, r, t);
+        if (a.y_dtype == Y_E4M3) {
+            unsigned w[V / 4];
+            to_e4m3<V>(t, inv, w);
+            bytes_store_n<V, false>((uint8_t*)a.y + yo + c, a.cols - c, w);
+        } else {
+            store_as<V, false>(a.y, a.y_dtype, yo + c, a.cols - c, t);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward
+// t of one chunk: from the tensor, or from the checkpoint
+template <int V, bool AL>
+__device__ __forceinline__ void stream_load(const RmsBwd& a, int row, int c, int n, float (&t)[V]) {
+    if (a.q) {
+        unsigned w[V / 4];
+        bytes_load_n<V, AL>(a.q + (size_t)row * a.cols + c, n, w);
+        const unsigned code = n > 0 ? a.code[(size_t)row * a.gpr + (c >> 5)] : 1u;
+        act8_dequant<V>(w, code, t);
+        if (n < V) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) t[j] = j < n ? t[j] : 0.f;
+        }
+    } else {
+        load_as<V, AL>(a.x, a.x_dtype, (size_t)row * a.ldx + c, n, t);
+    }
+}
+
+// Workgroups walk rows (nblk of them side by side); a lane keeps its columns' share of dgamma over all its rows in
+// registers, the workgroup writes one row of partial sums and rms_dgamma_kernel adds those in a fixed order.
+template <typename TDY, int V, int WPR, int NV, bool AL>
+__global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
+    constexpr int T = 64 * WPR;
+    __shared__ float red[2][4];
+    extern __shared__ float fold[];             // WPR == 1: [4][cols]
+    const int wave = threadIdx.x >> 6;
+    const int slot = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int stride = WPR == 1 ? a.nblk * 4 : a.nblk;
+    float g[NV][V], acc[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * T + slot) * V;
+        vec_load_n<float, V, AL>(a.gamma + c, a.cols - c, g[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[i][j] = 0.f;
+    }
+    int turn = 0;
+    for (int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x; row < a.rows; row += stride, turn ^= 1) {
+        const TDY* dy = (const TDY*)a.dy + (size_t)row * a.ldy;
+        float b[NV][V], h[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            vec_load_n<TDY, V, AL>(dy + c, a.cols - c, b[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            stream_load<V, AL>(a, row, c, a.cols - c, h[i]);
+        }
+        const float r = a.rstd[row];
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h[i][j] *= r;
+                acc[i][j] = fmaf(b[i][j], h[i][j], acc[i][j]);
+                b[i][j] *= g[i][j];
+                s = fmaf(b[i][j], h[i][j], s);
+            }
+        const float m = row_sum<WPR>(s, red[turn]) / (float)a.cols;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V, n = a.cols - c;
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = r * (b[i][j] - h[i][j] * m);
+            if (a.dres) {
+                float d[V];
+                load_as<V, AL>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, n, d);
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] += d[j];
+            }
+            store_as<V, AL>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, n, o);
+        }
+    }
+    float* part = a.part + (size_t)blockIdx.x * a.cols;
+    if constexpr (WPR == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (c + j < a.cols) fold[wave * a.cols + c + j] = acc[i][j];
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.cols; c += 256)
+            part[c] = (fold[c] + fold[a.cols + c]) + (fold[2 * a.cols + c] + fold[3 * a.cols + c]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * T + slot) * V;
+            vec_store_n<float, V, AL>(part + c, a.cols - c, acc[i]);
+        }
+    }
+}
+
+// any width: dx by one workgroup per row, two walks; dgamma by columns, a thread per column and chunk of rows
+template <typename TDY>
+__global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
+    constexpr int V = 8;
+    __shared__ float red[4];
+    const int row = blockIdx.x;
+    const TDY* dy = (const TDY*)a.dy + (size_t)row * a.ldy;
+    const float r = a.rstd[row];
+    auto chunk = [&](int c, float (&b)[V], float (&h)[V]) __attribute__((always_inline)) {
+        float g[V];
+        vec_load_n<TDY, V, false>(dy + c, a.cols - c, b);
+        vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
+        stream_load<V, false>(a, row, c, a.cols - c, h);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            b[j] *= g[j];
+            h[j] *= r;
+        }
+    };
+    float b[V], h[V], s = 0.f;
+    for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
+        chunk(c, b, h);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s = fmaf(b[j], h[j], s);
+    }
+    const float m = row_sum<4>(s, red) / (float)a.cols;
+    for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
+        chunk(c, b, h);
+#pragma unroll
+        for (int j = 0; j < V; ++j) b[j] = r * (b[j] - h[j] * m);
+        if (a.dres) {
+            float d[V];
+            load_as<V, false>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, a.cols - c, d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[j] += d[j];
+        }
+        store_as<V, false>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, a.cols - c, b);
+    }
+}
+// Every dy and t it reads was read by rms_bwd_long_kernel too; dx must therefore not overwrite dy (the entry point refuses
+// dx == dy for these widths).
+template <typename TDY>
+__global__ __launch_bounds__(256) void rms_dgamma_long_kernel(const RmsBwd a) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.cols) return;
+    float s = 0.f;
+    for (int row = blockIdx.y; row < a.rows; row += a.nblk) {
+        float t[1];
+        if (a.q) {
+            const float step = act8_step(a.code[(size_t)row * a.gpr + (c >> 5)]);
+            t[0] = (float)(int8_t)a.q[(size_t)row * a.cols + c] * step;
+        } else {
+            load_as<1, false>(a.x, a.x_dtype, (size_t)row * a.ldx + c, 1, t);
+        }
+        s = fmaf(to_f32<TDY>(((const TDY*)a.dy)[(size_t)row * a.ldy + c]), t[0] * a.rstd[row], s);
+    }
+    a.part[(size_t)blockIdx.y * a.cols + c] = s;
+}
+
+// dgamma[c] = sum of nparts rows of partial sums: 32 columns x 32 row lanes per workgroup, joined in a fixed order
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restrict__ part, float* __restrict__ out, int nparts,
+                                                          int cols) {
+    __shared__ float red[32][33];
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + cl;
+    float s = 0.f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int p = rl; p < nparts; p += 32) s += part[(size_t)p * cols + c];
+    }
+    red[rl][cl] = s;
+    __syncthreads();
+    if (rl == 0 && c < cols) {
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s += red[k][cl];
+        out[c] = s;
+    }
+}
+
+// ------------------------------------------------------------------ dispatch
+#define RMS_LONG 8192                           /* widest row kept in the registers of one workgroup */
+
+template <typename TX, int V, bool AL> void rms_fwd_launch(const RmsFwd& a, hipStream_t s) {
+    const dim3 wave((unsigned)((a.rows + 3) / 4)), wg((unsigned)a.rows), block(256);
+    const int chunks = (a.cols + V - 1) / V;
+#define RMS_FWD(W, N) hipLaunchKernelGGL((rms_fwd_kernel<TX, V, W, N, AL>), W == 1 ? wave : wg, block, 0, s, a)
+    if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
+        if (chunks <= 64) RMS_FWD(1, 1);
+        else if (chunks <= 128) RMS_FWD(1, 2);
+        else if (chunks <= 192) RMS_FWD(1, 3);
+        else if (chunks <= 256) RMS_FWD(1, 4);
+        else if (chunks <= 512) RMS_FWD(4, 2);
+        else if (chunks <= 1024) RMS_FWD(4, 4);
+        else RMS_FWD(4, 8);
+    } else {
+        if (chunks <= 64) RMS_FWD(1, 1);
+        else if (chunks <= 128) RMS_FWD(1, 2);
+        else if (chunks <= 256) RMS_FWD(4, 1);
+        else if (chunks <= 512) RMS_FWD(4, 2);
+        else RMS_FWD(4, 4);
+    }
+#undef RMS_FWD
+}
+template <typename TDY, int V, bool AL> void rms_bwd_launch(const RmsBwd& a, hipStream_t s) {
+    const dim3 grid((unsigned)a.nblk), block(256);
+    const int chunks = (a.cols + V - 1) / V;
+    const size_t lds = (size_t)16 * a.cols;     // WPR == 1: at most 16 KB
+#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, V, W, N, AL>), grid, block, W == 1 ? lds : 0, s, a)
+    if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
+        if (chunks <= 64) RMS_BWD(1, 1);
+        else if (chunks <= 128) RMS_BWD(1, 2);
+        else if (chunks <= 192) RMS_BWD(1, 3);
+        else if (chunks <= 256) RMS_BWD(1, 4);
+        else if (chunks <= 512) RMS_BWD(4, 2);
+        else if (chunks <= 1024) RMS_BWD(4, 4);
+        else RMS_BWD(4, 8);
+    } else {
+        if (chunks <= 64) RMS_BWD(1, 1);
+        else if (chunks <= 128) RMS_BWD(1, 2);
+        else if (chunks <= 256) RMS_BWD(4, 1);
+        else if (chunks <= 512) RMS_BWD(4, 2);
+        else RMS_BWD(4, 4);
+    }
+#undef RMS_BWD
+}
+
+template <typename TX> void rms_fwd_any(const RmsFwd& a, bool al, hipStream_t s) {
+    constexpr int V = sizeof(TX) == 4 ? 4 : 8;
+    if (a.cols > RMS_LONG) hipLaunchKernelGGL((rms_fwd_long_kernel<TX>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    else if (al) rms_fwd_launch<TX, V, true>(a, s);
+    else rms_fwd_launch<TX, V, false>(a, s);
+}
+template <typename TDY> void rms_bwd_any(const RmsBwd& a, bool al, hipStream_t s) {
+    constexpr int V = sizeof(TDY) == 4 ? 4 : 8;
+    if (a.cols > RMS_LONG) {
+        hipLaunchKernelGGL((rms_dgamma_long_kernel<TDY>), dim3((unsigned)((a.cols + 255) / 256), (unsigned)a.nblk), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((rms_bwd_long_kernel<TDY>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    } else if (al) {
+        rms_bwd_launch<TDY, V, true>(a, s);
+    } else {
+        rms_bwd_launch<TDY, V, false>(a, s);
+    }
+}
+
+// may rows of this tensor be read in whole aligned vectors of V elements?
+bool rows_aligned(const void* p, int64_t ld, size_t esz, int V) {
+    const size_t vec = esz * V < 16 ? esz * V : 16;
+    return p == nullptr || ((uintptr_t)p % vec == 0 && ((size_t)ld * esz) % vec == 0);
+}
+bool any_float(int dt) { return dt == BF_F32 || bf_is_half(dt); }
+
+int rms_fwd(const char* name, RmsFwd& a, int x_dtype, bf_stream_t stream) {
+    BF_REQUIRE(any_float(x_dtype), BF_EINVAL, "%s: bad x_dtype %d", name, x_dtype);
+    BF_REQUIRE(!a.delta || any_float(a.d_dtype), BF_EINVAL, "%s: bad delta_dtype %d", name, a.d_dtype);
+    BF_REQUIRE(a.rows >= 0 && a.cols > 0, BF_EINVAL, "%s: bad shape (rows=%d cols=%d)", name, a.rows, a.cols);
+    BF_REQUIRE(a.ldx >= a.cols && (!a.delta || a.ldd >= a.cols) && (!a.x_out || a.ldo >= a.cols), BF_EINVAL,
+               "%s: a leading dimension is under cols=%d", name, a.cols);
+    BF_REQUIRE((a.q == nullptr) == (a.code == nullptr), BF_EINVAL, "%s: a checkpoint is q and code, or neither", name);
+    BF_REQUIRE(a.eps >= 0.f, BF_EINVAL, "%s: eps must not be negative", name);
+    if (a.rows == 0) return BF_OK;
+    BF_REQUIRE(a.x && a.gamma && a.y && (a.y_dtype != Y_E4M3 || a.y_scale), BF_EINVAL, "%s: null pointer", name);
+    const size_t xs = bf_dtype_size(x_dtype), ds = bf_dtype_size(a.d_dtype), ys = a.y_dtype == Y_E4M3 ? 1 : bf_dtype_size(a.y_dtype);
+    BF_REQUIRE((uintptr_t)a.x % xs == 0 && (uintptr_t)a.x_out % xs == 0 && (uintptr_t)a.delta % ds == 0 && (uintptr_t)a.y % ys == 0 &&
+               (uintptr_t)a.gamma % 4 == 0 && (uintptr_t)a.rstd % 4 == 0 && (uintptr_t)a.y_scale % 4 == 0, BF_EALIGN,
+               "%s: a tensor is not aligned to its element", name);
+    a.gpr = (a.cols + ACT8_GROUP - 1) / ACT8_GROUP;
+    const int V = x_dtype == BF_F32 ? 4 : 8;
+    const bool al = a.cols % V == 0 && rows_aligned(a.x, a.ldx, xs, V) && rows_aligned(a.delta, a.ldd, ds, V) &&
+                    rows_aligned(a.x_out, a.ldo, xs, V) && rows_aligned(a.y, a.cols, ys, V) && rows_aligned(a.q, a.cols, 1, V) &&
+                    rows_aligned(a.gamma, a.cols, 4, V);
+    hipStream_t s = (hipStream_t)stream;
+    if (x_dtype == BF_F32) rms_fwd_any<float>(a, al, s);
+    else if (x_dtype == BF_BF16) rms_fwd_any<bf16_t>(a, al, s);
+    else rms_fwd_any<f16_t>(a, al, s);
+    BF_CHECK_LAUNCH(name);
+    return BF_OK;
+}
+
+}  // namespace
+
+extern "C" int bf_rmsnorm_fwd(const void* x, int64_t ldx, int x_dtype, const void* delta, int64_t ld_delta, int delta_dtype,
+                              const float* gamma, void* x_out, int64_t ld_out, void* y, int y_dtype, float* rstd, void* q,
+                              void* code, int rows, int cols, float eps, bf_stream_t stream) {
+    BF_REQUIRE(any_float(y_dtype), BF_EINVAL, "bf_rmsnorm_fwd: bad y_dtype %d", y_dtype);
+    RmsFwd a = {x, ldx, delta, ld_delta, delta_dtype, gamma, x_out, ld_out, y, y_dtype, nullptr, rstd, (uint8_t*)q,
+                (uint8_t*)code, rows, cols, 0, eps};
+    return rms_fwd("bf_rmsnorm_fwd", a, x_dtype, stream);
+}
+
+extern "C" int bf_rmsnorm_fwd_fp8(const void* x, int64_t ldx, int x_dtype, const void* delta, int64_t ld_delta, int delta_dtype,
+                                  const float* gamma, void* x_out, int64_t ld_out, void* y_fp8, float* row_scale, float* rstd,
+                                  void* q, void* code, int rows, int cols, float eps, bf_stream_t stream) {
+    RmsFwd a = {x, ldx, delta, ld_delta, delta_dtype, gamma, x_out, ld_out, y_fp8, Y_E4M3, row_scale, rstd, (uint8_t*)q,
+                (uint8_t*)code, rows, cols, 0, eps};
+    return rms_fwd("bf_rmsnorm_fwd_fp8", a, x_dtype, stream);
+}
+
+extern "C" int bf_rmsnorm_bwd_parts(int rows, int cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    if (cols > RMS_LONG) return rows < 64 ? rows : 64;
+    // a row per wave: up to 1 024 workgroups of four rows side by side; a row per workgroup: half as many partial rows, each
+    // up to 32 KB
+    if (cols <= 1024) return (rows + 3) / 4 < 1024 ? (rows + 3) / 4 : 1024;
+    return rows < 512 ? rows : 512;
+}
+
+extern "C" int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const void* x, int64_t ldx, int x_dtype, const void* q,
+                              const void* code, const float* gamma, const float* rstd, const void* dres, int64_t ld_dres,
+                              void* dx, int dx_dtype, float* dgamma, float* parts_ws, int rows, int cols, bf_stream_t stream) {
+    const char* name = "bf_rmsnorm_bwd";
+    BF_REQUIRE(any_float(dy_dtype) && any_float(dx_dtype), BF_EINVAL, "%s: bad dy_dtype %d or dx_dtype %d", name, dy_dtype, dx_dtype);
+    BF_REQUIRE(rows >= 0 && cols > 0, BF_EINVAL, "%s: bad shape (rows=%d cols=%d)", name, rows, cols);
+    BF_REQUIRE((q == nullptr) == (code == nullptr), BF_EINVAL, "%s: a checkpoint is q and code, or neither", name);
+    BF_REQUIRE(dgamma && (uintptr_t)dgamma % 4 == 0, BF_EINVAL, "%s: null dgamma", name);
+    hipStream_t s = (hipStream_t)stream;
+    if (rows == 0) {
+        hipError_t e = bf_zero_f32_async(dgamma, (size_t)cols, s);
+        BF_REQUIRE(e == hipSuccess, BF_ELAUNCH, "%s: launch failed", name);
+        return BF_OK;
+    }
+    BF_REQUIRE((x == nullptr) != (q == nullptr), BF_EINVAL, "%s: the stream is x, or a checkpoint q / code: exactly one", name);
+    BF_REQUIRE(!x || any_float(x_dtype), BF_EINVAL, "%s: bad x_dtype %d", name, x_dtype);
+    BF_REQUIRE(dy && gamma && rstd && dx && parts_ws, BF_EINVAL, "%s: null pointer", name);
+    BF_REQUIRE(ld_dy >= cols && (!x || ldx >= cols) && (!dres || ld_dres >= cols), BF_EINVAL,
+               "%s: a leading dimension is under cols=%d", name, cols);
+    BF_REQUIRE(cols <= RMS_LONG || dx != dy, BF_EINVAL, "%s: dx may be dy up to %d columns only", name, RMS_LONG);
+    BF_REQUIRE(dx != dy || (ld_dy == cols && dx_dtype == dy_dtype), BF_EINVAL, "%s: dx may be dy only where their rows coincide", name);
+    BF_REQUIRE(dx != dres || ld_dres == cols, BF_EINVAL, "%s: dx may be dres only where their rows coincide", name);
+    const size_t ys = bf_dtype_size(dy_dtype), xs = bf_dtype_size(x_dtype), os = bf_dtype_size(dx_dtype);
+    BF_REQUIRE((uintptr_t)dy % ys == 0 && (!x || (uintptr_t)x % xs == 0) && (uintptr_t)dres % os == 0 && (uintptr_t)dx % os == 0 &&
+               (uintptr_t)gamma % 4 == 0 && (uintptr_t)rstd % 4 == 0 && (uintptr_t)parts_ws % 4 == 0, BF_EALIGN,
+               "%s: a tensor is not aligned to its element", name);
+    RmsBwd a = {dy, ld_dy, x, ldx, x_dtype, (const uint8_t*)q, (const uint8_t*)code, gamma, rstd, dres, ld_dres, dx, dx_dtype,
+                parts_ws, rows, cols, (cols + ACT8_GROUP - 1) / ACT8_GROUP, bf_rmsnorm_bwd_parts(rows, cols)};
+    const int V = dy_dtype == BF_F32 ? 4 : 8;
+    const bool al = cols % V == 0 && rows_aligned(dy, ld_dy, ys, V) && (!x || rows_aligned(x, ldx, xs, V)) &&
+                    rows_aligned(q, cols, 1, V) && rows_aligned(dres, ld_dres, os, V) && rows_aligned(dx, cols, os, V) &&
+                    rows_aligned(gamma, cols, 4, V) && rows_aligned(parts_ws, cols, 4, V);
+    if (a.nblk == 1) a.part = dgamma;           // one row of partial sums is the result
+    if (dy_dtype == BF_F32) rms_bwd_any<float>(a, al && rows_aligned(a.part, cols, 4, V), s);
+    else if (dy_dtype == BF_BF16) rms_bwd_any<bf16_t>(a, al && rows_aligned(a.part, cols, 4, V), s);
+    else rms_bwd_any<f16_t>(a, al && rows_aligned(a.part, cols, 4, V), s);
+    BF_CHECK_LAUNCH(name);
+    if (a.nblk > 1) {
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, s, parts_ws, dgamma, a.nblk, cols);
+        BF_CHECK_LAUNCH(name);
+    }
+    return BF_OK;
+}

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_long, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_long, c_size_t, c_void_p
 
 # PyTorch-ROCm ships its own libamdhip64; it must be in the process BEFORE libbifold_hip.so so
 # that both resolve to ONE HIP runtime (device pointers and streams cross this boundary).
@@ -175,6 +175,23 @@ PROTOTYPES = {
     "bf_heatmap_pick": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "bf_gaussian_targets": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_double, c_int,
                                     c_void_p]),
+    "bf_act8_pack": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "bf_act8_unpack": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_void_p]),
+    "bf_act8_gelu_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int, c_void_p]),
+    "bf_act8_gelu_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64, c_int,
+                                 c_void_p]),
+    "bf_rmsnorm_fwd": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int,
+                               c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]),
+    "bf_rmsnorm_fwd_fp8": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]),
+    "bf_rmsnorm_bwd_parts": (c_int, [c_int, c_int]),
+    "bf_rmsnorm_bwd": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "bf_embed_scaled_fwd": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_int, c_int, c_int, c_void_p,
+                                    c_void_p]),
+    "bf_embed_scaled_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "bf_embed_scaled_bwd": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 

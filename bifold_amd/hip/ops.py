@@ -1056,3 +1056,282 @@ def gemm_fp8(a8: torch.Tensor, a_scale: torch.Tensor, b8: torch.Tensor, b_scale:
     if span is not None:
         span.close()
     return out
+
+
+# ----------------------------------------------------------------------------- rows of any leading dimension
+def _here(*named) -> None:
+    """Every (tensor, name) lives on the current device: the launch goes to that device's stream."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t, name in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
+        if t.device.index != dev:
+            raise RuntimeError(f"{name} lives on {t.device}, the current device is cuda:{dev}")
+
+
+def _row_layout(t: torch.Tensor, name: str):
+    """(rows, cols, leading dimension) of a tensor whose last dimension is a row: contiguous, or 2-D with unit inner stride."""
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise RuntimeError(f"{name} needs a last dimension of at least one element, got {tuple(t.shape)}")
+    cols = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // cols, cols, cols
+    if t.dim() == 2 and (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or t.shape[0] == 1):
+        return t.shape[0], cols, t.stride(0) if t.shape[0] > 1 else cols
+    raise RuntimeError(f"{name} must be contiguous, or 2-D with unit inner stride and rows that do not overlap, got "
+                       f"{tuple(t.shape)} {t.stride()}")
+
+
+def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do the address ranges of two tensors meet?  (Strided views count from their first to their last element.)"""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+
+
+# ----------------------------------------------------------------------------- 8-bit activation checkpoints
+ACT8_GROUP = 32
+_GELUS = (L.ACT_QUICK_GELU, L.ACT_ERF_GELU, L.ACT_TANH_GELU)
+Checkpoint = Tuple[torch.Tensor, torch.Tensor]
+
+
+def _act8_empty(shape, device) -> Checkpoint:
+    groups = (shape[-1] + ACT8_GROUP - 1) // ACT8_GROUP
+    return (torch.empty(shape, dtype=torch.int8, device=device),
+            torch.empty(tuple(shape[:-1]) + (groups,), dtype=torch.uint8, device=device))
+
+
+def _act8_parts(kept: Checkpoint):
+    q, code = kept
+    if q.dtype != torch.int8 or code.dtype != torch.uint8 or q.dim() < 1 or q.shape[-1] == 0 or not q.is_contiguous() \
+            or not code.is_contiguous() or q.shape[:-1] != code.shape[:-1] \
+            or code.shape[-1] != (q.shape[-1] + ACT8_GROUP - 1) // ACT8_GROUP:
+        raise RuntimeError("a checkpoint is (q int8 [..., cols], code uint8 [..., ceil(cols / 32)]), both contiguous, got "
+                           f"{q.dtype} {tuple(q.shape)}, {code.dtype} {tuple(code.shape)}")
+    return q, code
+
+
+def act8_pack(x: torch.Tensor) -> Checkpoint:
+    """The 8-bit checkpoint (q int8, code uint8) of x [..., cols], 33/32 bytes per element: groups of 32 columns share a
+    power of two 2^e (code = e + 127), q = round(x 2^-e); see bf_act8_pack."""
+    rows, cols, ld = _row_layout(x, "x")
+    _here((x, "x"))
+    q, code = _act8_empty(x.shape, x.device)
+    check(lib.bf_act8_pack(x.data_ptr(), ld, dtype_code(x), q.data_ptr(), code.data_ptr(), rows, cols, _stream()),
+          "bf_act8_pack")
+    return q, code
+
+
+def act8_unpack(kept: Checkpoint, dtype: torch.dtype, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The tensor a checkpoint stands for: q 2^e (exact in fp32 and bf16; NaN throughout a group that was not finite)."""
+    q, code = _act8_parts(kept)
+    if out is None:
+        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype:
+        raise RuntimeError(f"act8_unpack: out must be {dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+    rows, cols, ld = _row_layout(out, "out")
+    _here((q, "q"), (code, "code"), (out, "out"))
+    check(lib.bf_act8_unpack(q.data_ptr(), code.data_ptr(), out.data_ptr(), ld, dtype_code(out), rows, cols, _stream()),
+          "bf_act8_unpack")
+    return out
+
+
+def act8_gelu_fwd(pre: torch.Tensor, act: int) -> Tuple[torch.Tensor, Checkpoint]:
+    """(y, checkpoint of pre) with y = act(pre) in pre's dtype, in one pass; act: ACT_QUICK_GELU, ACT_ERF_GELU or
+    ACT_TANH_GELU."""
+    rows, cols, ld = _row_layout(pre, "pre")
+    _here((pre, "pre"))
+    y = torch.empty(pre.shape, dtype=pre.dtype, device=pre.device)
+    q, code = _act8_empty(pre.shape, pre.device)
+    check(lib.bf_act8_gelu_fwd(pre.data_ptr(), ld, y.data_ptr(), q.data_ptr(), code.data_ptr(), dtype_code(pre), act, rows, cols,
+                               _stream()), "bf_act8_gelu_fwd")
+    return y, (q, code)
+
+
+def act8_gelu_bwd(dy: torch.Tensor, kept: Checkpoint, act: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dpre = dy act'(what the checkpoint stands for), in dy's dtype.  `out` may be dy itself."""
+    q, code = _act8_parts(kept)
+    if dy.shape != q.shape:
+        raise RuntimeError(f"act8_gelu_bwd: dy {tuple(dy.shape)} does not match the checkpoint {tuple(q.shape)}")
+    rows, cols, ld = _row_layout(dy, "dy")
+    if out is None:
+        out = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    elif out.shape != dy.shape or out.dtype != dy.dtype or (_overlap(out, dy) and not _same_rows(out, dy)):
+        raise RuntimeError("act8_gelu_bwd: out has dy's shape and dtype, and is dy or memory of its own")
+    _, _, ldo = _row_layout(out, "out")
+    _here((dy, "dy"), (q, "q"), (code, "code"), (out, "out"))
+    check(lib.bf_act8_gelu_bwd(dy.data_ptr(), ld, q.data_ptr(), code.data_ptr(), out.data_ptr(), ldo, dtype_code(dy), act, rows,
+                               cols, _stream()), "bf_act8_gelu_bwd")
+    return out
+
+
+# ----------------------------------------------------------------------------- RMS norm
+def _rms_args(x, gamma, delta, x_out, write_x):
+    rows, cols, ldx = _row_layout(x, "x")
+    _vector(gamma, cols, "gamma")
+    ldd = d_dtype = ldo = 0
+    if delta is None:
+        if x_out is not None and x_out is not x:
+            raise RuntimeError("rmsnorm: x_out without a delta to add")
+        x_out = None
+    else:
+        if delta.shape != x.shape:
+            raise RuntimeError(f"rmsnorm: delta {tuple(delta.shape)} does not match x {tuple(x.shape)}")
+        _, _, ldd = _row_layout(delta, "delta")
+        d_dtype = dtype_code(delta)
+        if not write_x:
+            x_out = None
+        else:
+            if x_out is None:
+                x_out = x
+            elif x_out.shape != x.shape or x_out.dtype != x.dtype:
+                raise RuntimeError("rmsnorm: x_out has x's shape and dtype")
+            for t, name in ((x, "x"), (delta, "delta")):
+                if _overlap(x_out, t) and not _same_rows(x_out, t):
+                    raise RuntimeError(f"rmsnorm: x_out is {name} or memory of its own")
+            _, _, ldo = _row_layout(x_out, "x_out")
+    _here((x, "x"), (gamma, "gamma"), (delta, "delta"), (x_out, "x_out"))
+    return rows, cols, ldx, ldd, d_dtype, ldo, x_out
+
+
+def rmsnorm_fwd(x: torch.Tensor, gamma: torch.Tensor, out_dtype: torch.dtype, delta: Optional[torch.Tensor] = None,
+                x_out: Optional[torch.Tensor] = None, write_x: bool = True, save_stats: bool = False, eps: float = 1e-6,
+                checkpoint: bool = False):
+    """t = x + delta; y = t / sqrt(mean(t^2) + eps) * gamma over the last dimension.  x_out = t rounded to x's dtype: given,
+    or x itself (in place) when None, or not written (write_x=False; also without a delta).  `checkpoint`: also the 8-bit
+    checkpoint of t.  Returns (y, rstd or None, checkpoint or None)."""
+    rows, cols, ldx, ldd, d_dtype, ldo, x_out = _rms_args(x, gamma, delta, x_out, write_x)
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if save_stats else None
+    q, code = _act8_empty(x.shape, x.device) if checkpoint else (None, None)
+    check(lib.bf_rmsnorm_fwd(x.data_ptr(), ldx, dtype_code(x), _ptr(delta), ldd, d_dtype, gamma.data_ptr(), _ptr(x_out), ldo,
+                             y.data_ptr(), dtype_code(y), _ptr(rstd), _ptr(q), _ptr(code), rows, cols, eps, _stream()),
+          "bf_rmsnorm_fwd")
+    return y, rstd, (q, code) if checkpoint else None
+
+
+def rmsnorm_fwd_fp8(x: torch.Tensor, gamma: torch.Tensor, delta: Optional[torch.Tensor] = None,
+                    x_out: Optional[torch.Tensor] = None, write_x: bool = True, save_stats: bool = False, eps: float = 1e-6,
+                    checkpoint: bool = False):
+    """rmsnorm_fwd with e4m3 output for ops.gemm_fp8: returns (y uint8, row scales fp32 [rows], rstd or None, checkpoint or
+    None); y ~= bytes * scale, scale = max |y| / 448 of the row."""
+    rows, cols, ldx, ldd, d_dtype, ldo, x_out = _rms_args(x, gamma, delta, x_out, write_x)
+    y = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if save_stats else None
+    q, code = _act8_empty(x.shape, x.device) if checkpoint else (None, None)
+    check(lib.bf_rmsnorm_fwd_fp8(x.data_ptr(), ldx, dtype_code(x), _ptr(delta), ldd, d_dtype, gamma.data_ptr(), _ptr(x_out),
+                                 ldo, y.data_ptr(), scale.data_ptr(), _ptr(rstd), _ptr(q), _ptr(code), rows, cols, eps,
+                                 _stream()), "bf_rmsnorm_fwd_fp8")
+    return y, scale, rstd, (q, code) if checkpoint else None
+
+
+def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dgamma_out: torch.Tensor,
+                dres: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dx = dres + d rmsnorm / dx (dy); dgamma_out [cols] is written.  `x`: the normed stream, a tensor or the checkpoint the
+    forward left; rstd: the forward's.  dx has dres's dtype (dy's without one); `out` may be dres or dy."""
+    rows, cols, ldy = _row_layout(dy, "dy")
+    _vector(gamma, cols, "gamma"), _vector(rstd, rows, "rstd"), _vector(dgamma_out, cols, "dgamma_out")
+    q = code = None
+    ldx = x_dtype = ldr = 0
+    if isinstance(x, torch.Tensor):
+        shape = x.shape
+        _, _, ldx = _row_layout(x, "x")
+        x_dtype = dtype_code(x)
+    else:
+        q, code = _act8_parts(x)
+        shape, x = q.shape, None
+    if shape != dy.shape or (dres is not None and dres.shape != dy.shape):
+        raise RuntimeError(f"rmsnorm_bwd: dy {tuple(dy.shape)}, x {tuple(shape)} and dres must have one shape")
+    dt = dy.dtype if dres is None else dres.dtype
+    if dres is not None:
+        _, _, ldr = _row_layout(dres, "dres")
+    if out is None:
+        out = torch.empty(dy.shape, dtype=dt, device=dy.device)
+    else:
+        if out.shape != dy.shape or out.dtype != dt or not out.is_contiguous():
+            raise RuntimeError(f"rmsnorm_bwd: out must be a contiguous {dt} tensor of dy's shape")
+        for t, name in ((dy, "dy"), (dres, "dres")):
+            if t is not None and _overlap(out, t) and not (_same_rows(out, t) and (name == "dres" or cols <= 8192)):
+                raise RuntimeError(f"rmsnorm_bwd: out is {name} (dy: up to 8192 columns) or memory of its own")
+        for t in (x, q, code, gamma, rstd, dgamma_out):
+            if t is not None and _overlap(out, t):
+                raise RuntimeError("rmsnorm_bwd: out must not overlap x, the checkpoint, gamma, rstd or dgamma_out")
+    _here((dy, "dy"), (x, "x"), (q, "q"), (code, "code"), (gamma, "gamma"), (rstd, "rstd"), (dres, "dres"), (out, "out"),
+          (dgamma_out, "dgamma_out"))
+    parts = torch.empty(lib.bf_rmsnorm_bwd_parts(rows, cols), cols, dtype=torch.float32, device=dy.device)
+    check(lib.bf_rmsnorm_bwd(dy.data_ptr(), ldy, dtype_code(dy), _ptr(x), ldx, x_dtype, _ptr(q), _ptr(code), gamma.data_ptr(),
+                             rstd.data_ptr(), _ptr(dres), ldr, out.data_ptr(), dtype_code(out), dgamma_out.data_ptr(),
+                             parts.data_ptr(), rows, cols, _stream()), "bf_rmsnorm_bwd")
+    return out
+
+
+# ----------------------------------------------------------------------------- scaled embedding and its gradient
+def _token_ids(tokens: torch.Tensor) -> int:
+    if tokens.dtype != torch.int32 or not tokens.is_contiguous():
+        raise TypeError(f"token ids must be a contiguous int32 tensor, got {tokens.dtype}")
+    return tokens.numel()
+
+
+def _flag(err_flag: Optional[torch.Tensor]) -> None:
+    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
+        raise TypeError("err_flag must be an int32 tensor of one element")
+
+
+def embed_scaled_fwd(tokens: torch.Tensor, table: torch.Tensor, scale: float, err_flag: Optional[torch.Tensor] = None,
+                     out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """out [tokens, cols] = scale * table[token].  A token outside the table reads row 0 and sets err_flag."""
+    n = _token_ids(tokens)
+    _flag(err_flag)
+    if table.dim() != 2 or not table.is_contiguous() or 0 in table.shape:
+        raise RuntimeError(f"embed_scaled_fwd: table must be a contiguous [vocab, cols] tensor, got {tuple(table.shape)}")
+    _here((tokens, "tokens"), (table, "table"), (err_flag, "err_flag"))
+    vocab, cols = table.shape
+    out = torch.empty(n, cols, dtype=out_dtype or table.dtype, device=table.device)
+    check(lib.bf_embed_scaled_fwd(tokens.data_ptr(), table.data_ptr(), dtype_code(table), out.data_ptr(), dtype_code(out),
+                                  scale, n, cols, vocab, _ptr(err_flag), _stream()), "bf_embed_scaled_fwd")
+    return out
+
+
+def embed_scaled_bwd(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float, err_flag: Optional[torch.Tensor] = None,
+                     padding_idx: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                     accumulate: bool = False) -> torch.Tensor:
+    """grad [vocab, cols] fp32 = scale * the sum of dy's rows per token, in a fixed order; rows of padding_idx and of tokens
+    outside the table (which set err_flag) are left out.  `accumulate`: add into `out`, touching the rows of tokens that
+    occur only."""
+    n = _token_ids(tokens)
+    _flag(err_flag)
+    rows, cols, ld = _row_layout(dy, "dy")
+    if rows != n:
+        raise RuntimeError(f"embed_scaled_bwd: {rows} rows of dy for {n} tokens")
+    if vocab <= 0 or (padding_idx is not None and not 0 <= padding_idx < vocab):
+        raise ValueError(f"embed_scaled_bwd: vocab={vocab}, padding_idx={padding_idx}")
+    if out is None:
+        if accumulate:
+            raise RuntimeError("accumulate needs an `out` to add into")
+        out = torch.empty(vocab, cols, dtype=torch.float32, device=dy.device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (vocab, cols) or not out.is_contiguous() or _overlap(out, dy):
+        raise RuntimeError(f"embed_scaled_bwd: out must be a contiguous float32 {(vocab, cols)} tensor apart from dy")
+    _here((dy, "dy"), (tokens, "tokens"), (out, "out"), (err_flag, "err_flag"))
+    need = lib.bf_embed_scaled_bwd_workspace_bytes(n, cols, vocab)
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    check(lib.bf_embed_scaled_bwd(dy.data_ptr(), ld, dtype_code(dy), tokens.data_ptr(), out.data_ptr(), scale, int(accumulate),
+                                  -1 if padding_idx is None else padding_idx, n, cols, vocab, _ptr(err_flag), _ptr(ws), need,
+                                  _stream()), "bf_embed_scaled_bwd")
+    return out

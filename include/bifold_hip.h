@@ -647,6 +647,61 @@ int bf_heatmap_pick(const float* heat, const float* mask, int32_t* xy, float* co
 int bf_gaussian_targets(const float* points, const int32_t* counts, float* heat, int n_maps,
                         int max_points, int size, double sigma, int strategy, bf_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits: what a training step keeps of an activation between its forward and its backward pass.
+ * (No reference counterpart: its autograd keeps every activation in fp32.  Entry points from here to the end of this block
+ * were added without a change of the ABI version: nothing that was there changed.)
+ *   A row of x [rows, cols] (rows ld elements apart) is cut into groups of 32 columns, the last possibly shorter.  A group
+ *   shares the power of two 2^e, e the smallest exponent >= -126 for which round(max |x| 2^-e) <= 127;
+ *     q [rows, cols] int8 = round(x 2^-e), ties to even      code [rows, ceil(cols / 32)] uint8 = e + 127
+ *   and x reads back as q 2^e: off by at most 2^(e-1) <= max |x| / 127.  A group with a NaN, an infinity or a magnitude of
+ *   255 * 2^119 or more has code 255 and reads back as NaN.
+ * dtype: BF_F32 / BF_BF16 / BF_F16 of x, pre, y, dy, dpre.  rows * ceil(cols / 32) * 4 < 2^32.  Pointers need the alignment
+ * of their element only; cols a multiple of 32, no gaps between rows and 16-byte alignment give the fast path.
+ *   gelu_fwd: y [rows, cols] = act(pre) and the checkpoint of pre, one pass.  act: BF_ACT_QUICK_GELU / _ERF_GELU / _TANH_GELU
+ *   gelu_bwd: dpre = dy act'(q 2^e); dpre may be dy (same leading dimension).
+ * ---------------------------------------------------------------------- */
+int bf_act8_pack(const void* x, int64_t ldx, int dtype, void* q, void* code, int64_t rows, int cols, bf_stream_t stream);
+int bf_act8_unpack(const void* q, const void* code, void* x, int64_t ldx, int dtype, int64_t rows, int cols, bf_stream_t stream);
+int bf_act8_gelu_fwd(const void* pre, int64_t ld_pre, void* y, void* q, void* code, int dtype, int act, int64_t rows, int cols,
+                     bf_stream_t stream);
+int bf_act8_gelu_bwd(const void* dy, int64_t ld_dy, const void* q, const void* code, void* dpre, int64_t ld_dpre, int dtype, int act,
+                     int64_t rows, int cols, bf_stream_t stream);
+
+/* Root-mean-square norm with the residual's addition:  t = x + delta;  r = 1 / sqrt(mean(t^2) + eps);  y = t r gamma.
+ *   x [rows, ldx] any float type; delta [rows, ld_delta] any float type or NULL; x_out [rows, ld_out] = t rounded to x's type,
+ *   or NULL (may be x); y [rows, cols]; rstd [rows] = r, or NULL; q / code = the 8-bit checkpoint of t, or both NULL.
+ *   t enters y, r and the checkpoint unrounded; statistics are fp32.
+ * _fp8: y_fp8 = e4m3(y / row_scale), row_scale = max |y| / 448 per row (1 for a row of zeros, NaN for a row with a NaN or an
+ *   infinity): bf_gemm_fp8's operand, as bf_layernorm_fwd_fp8 writes it.
+ * bwd:  h = t r;  b = dy gamma;  dx = dres + r (b - h mean(b h));  dgamma [cols] = sum over rows of dy h (overwritten; summed
+ *   in a fixed order).  The stream t is x, or a checkpoint q / code with x = NULL; dres (of dx's type) may be NULL; dx may be
+ *   dres, and up to 8 192 columns dy, where their rows coincide.  parts_ws: bf_rmsnorm_bwd_parts(rows, cols) * cols floats. */
+int bf_rmsnorm_fwd(const void* x, int64_t ldx, int x_dtype, const void* delta, int64_t ld_delta, int delta_dtype, const float* gamma,
+                   void* x_out, int64_t ld_out, void* y, int y_dtype, float* rstd, void* q, void* code, int rows, int cols,
+                   float eps, bf_stream_t stream);
+int bf_rmsnorm_fwd_fp8(const void* x, int64_t ldx, int x_dtype, const void* delta, int64_t ld_delta, int delta_dtype,
+                       const float* gamma, void* x_out, int64_t ld_out, void* y_fp8, float* row_scale, float* rstd, void* q,
+                       void* code, int rows, int cols, float eps, bf_stream_t stream);
+int bf_rmsnorm_bwd_parts(int rows, int cols);
+int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const void* x, int64_t ldx, int x_dtype, const void* q,
+                   const void* code, const float* gamma, const float* rstd, const void* dres, int64_t ld_dres, void* dx,
+                   int dx_dtype, float* dgamma, float* parts_ws, int rows, int cols, bf_stream_t stream);
+
+/* Embedding lookup with scaling, and the gradient of its table.
+ *   fwd: out [n, cols] = scale * table[tokens[i], :]  (table [vocab, cols]).  A token outside the table sets err_flag (may be
+ *        NULL) and reads row 0, as bf_embed_tokens does.
+ *   bwd: grad [vocab, cols] fp32 = scale * the sum of the rows of dy [n, ld_dy] that share the token; accumulate != 0 adds to
+ *        what is there instead and touches the rows of tokens that occur only.  Rows of the token padding_idx (-1: none) and
+ *        of tokens outside the table (which set err_flag) are left out.  Sums are fp32, in a fixed order.
+ *        workspace: bf_embed_scaled_bwd_workspace_bytes (0 for n <= 512), 16-byte aligned; n <= 2^30. */
+int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int table_dtype, void* out, int out_dtype, float scale, int n,
+                        int cols, int vocab, int* err_flag, bf_stream_t stream);
+size_t bf_embed_scaled_bwd_workspace_bytes(int n, int cols, int vocab);
+int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const int32_t* tokens, float* grad, float scale, int accumulate,
+                        int padding_idx, int n, int cols, int vocab, int* err_flag, void* workspace, size_t workspace_bytes,
+                        bf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

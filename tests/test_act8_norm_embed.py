@@ -1,0 +1,163 @@
+"""Host side of the 8-bit activation checkpoints, the RMS norm and the scaled embedding: what the entry points refuse, before
+any launch, and the workspace sizes they ask for."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def L():
+    from bifold_amd.hip import lib
+    return lib
+
+
+PTR = 4096                                     # an aligned address nothing reads: every call below is refused
+
+
+def refused(L, rc, code, text):
+    assert rc == code, (rc, L.lib.bf_last_error())
+    assert text.encode() in L.lib.bf_last_error(), L.lib.bf_last_error()
+
+
+def test_act8_refusals(L):
+    lib = L.lib
+    refused(L, lib.bf_act8_pack(PTR, 64, 7, PTR, PTR, 4, 64, None), -1, "bad dtype")
+    refused(L, lib.bf_act8_pack(PTR, 64, L.F32, PTR, PTR, 4, 0, None), -1, "bad shape")
+    refused(L, lib.bf_act8_pack(PTR, 64, L.F32, PTR, PTR, -1, 64, None), -1, "bad shape")
+    refused(L, lib.bf_act8_pack(PTR, 63, L.F32, PTR, PTR, 4, 64, None), -1, "leading dimension")
+    refused(L, lib.bf_act8_pack(None, 64, L.F32, PTR, PTR, 4, 64, None), -1, "null")
+    refused(L, lib.bf_act8_pack(PTR, 64, L.F32, PTR, None, 4, 64, None), -1, "null")
+    refused(L, lib.bf_act8_pack(PTR + 2, 64, L.F32, PTR, PTR, 4, 64, None), -2, "aligned")
+    refused(L, lib.bf_act8_pack(PTR, 32, L.F16, PTR, PTR, 1 << 30, 32, None), -1, "2^35")
+    refused(L, lib.bf_act8_unpack(PTR, PTR, PTR, 63, L.F16, 4, 64, None), -1, "leading dimension")
+    refused(L, lib.bf_act8_unpack(PTR, PTR, PTR + 1, 64, L.F16, 4, 64, None), -2, "aligned")
+    for act in (L.ACT_NONE, 3, 5, 99):
+        refused(L, lib.bf_act8_gelu_fwd(PTR, 64, PTR, PTR, PTR, L.F16, act, 4, 64, None), -1, "act must be")
+        refused(L, lib.bf_act8_gelu_bwd(PTR, 64, PTR, PTR, PTR, 64, L.F16, act, 4, 64, None), -1, "act must be")
+    assert lib.bf_act8_pack(None, 64, L.F32, None, None, 0, 64, None) == 0         # no rows: nothing to do
+
+
+def test_rmsnorm_refusals(L):
+    lib = L.lib
+
+    def fwd(x=PTR, ldx=64, xd=L.F32, delta=None, ldd=0, dd=0, gamma=PTR, xo=None, ldo=0, y=PTR, yd=L.F32, rstd=None, q=None,
+            code=None, rows=4, cols=64, eps=1e-6):
+        return lib.bf_rmsnorm_fwd(x, ldx, xd, delta, ldd, dd, gamma, xo, ldo, y, yd, rstd, q, code, rows, cols, eps, None)
+
+    refused(L, fwd(xd=5), -1, "x_dtype")
+    refused(L, fwd(yd=3), -1, "y_dtype")
+    refused(L, fwd(delta=PTR, ldd=64, dd=9), -1, "delta_dtype")
+    refused(L, fwd(cols=0), -1, "bad shape")
+    refused(L, fwd(ldx=60), -1, "leading dimension")
+    refused(L, fwd(delta=PTR, ldd=63), -1, "leading dimension")
+    refused(L, fwd(delta=PTR, ldd=64, xo=PTR, ldo=3), -1, "leading dimension")
+    refused(L, fwd(q=PTR), -1, "checkpoint")
+    refused(L, fwd(eps=-1.0), -1, "eps")
+    refused(L, fwd(gamma=None), -1, "null")
+    refused(L, fwd(y=PTR + 1), -2, "aligned")
+    refused(L, lib.bf_rmsnorm_fwd_fp8(PTR, 64, L.F32, None, 0, 0, PTR, None, 0, PTR, None, None, None, None, 4, 64, 1e-6, None),
+            -1, "null")
+    assert fwd(rows=0, x=None, y=None) == 0
+
+    def bwd(dy=PTR, ldy=64, dyd=L.F16, x=PTR, ldx=64, xd=L.F32, q=None, code=None, gamma=PTR, rstd=PTR, dres=None, ldr=0,
+            dx=2 * PTR, dxd=L.F16, dg=PTR, ws=PTR, rows=4, cols=64):
+        return lib.bf_rmsnorm_bwd(dy, ldy, dyd, x, ldx, xd, q, code, gamma, rstd, dres, ldr, dx, dxd, dg, ws, rows, cols, None)
+
+    refused(L, bwd(dyd=4), -1, "dy_dtype")
+    refused(L, bwd(xd=4), -1, "x_dtype")
+    refused(L, bwd(x=None), -1, "exactly one")
+    refused(L, bwd(q=PTR, code=PTR), -1, "exactly one")
+    refused(L, bwd(code=PTR), -1, "checkpoint")
+    refused(L, bwd(dg=None), -1, "dgamma")
+    refused(L, bwd(ws=None), -1, "null")
+    refused(L, bwd(ldy=63), -1, "leading dimension")
+    refused(L, bwd(dx=PTR, ldy=72), -1, "rows coincide")
+    refused(L, bwd(dx=PTR, dxd=L.F32), -1, "rows coincide")
+    refused(L, bwd(dres=2 * PTR, ldr=72), -1, "rows coincide")
+    refused(L, bwd(dx=PTR, cols=8200, ldy=8200, ldx=8200), -1, "8192")
+    refused(L, bwd(rstd=PTR + 1), -2, "aligned")
+    assert [lib.bf_rmsnorm_bwd_parts(r, c) for r, c in ((0, 64), (1, 64), (5, 64), (10 ** 6, 64), (7, 4096), (9000, 4096),
+                                                         (9000, 9000))] == [0, 1, 2, 1024, 7, 512, 64]
+
+
+def test_embedding_refusals(L):
+    lib = L.lib
+    refused(L, lib.bf_embed_scaled_fwd(PTR, PTR, 6, PTR, L.F32, 1.0, 4, 64, 100, None, None), -1, "dtype")
+    refused(L, lib.bf_embed_scaled_fwd(PTR, PTR, L.F32, PTR, L.F32, 1.0, 4, 64, 0, None, None), -1, "bad shape")
+    refused(L, lib.bf_embed_scaled_fwd(PTR, None, L.F32, PTR, L.F32, 1.0, 4, 64, 100, None, None), -1, "null")
+    refused(L, lib.bf_embed_scaled_fwd(PTR + 2, PTR, L.F32, PTR, L.F32, 1.0, 4, 64, 100, None, None), -2, "aligned")
+    refused(L, lib.bf_embed_scaled_fwd(PTR, PTR, L.F32, PTR, L.F32, 1.0, 1 << 30, 4096, 100, None, None), -1, "too large")
+
+    def bwd(dy=PTR, ld=64, dt=L.F16, ids=PTR, grad=PTR, n=1000, cols=64, vocab=100, ws=PTR, size=None, acc=1):
+        size = lib.bf_embed_scaled_bwd_workspace_bytes(n, cols, vocab) if size is None else size
+        return lib.bf_embed_scaled_bwd(dy, ld, dt, ids, grad, 1.0, acc, -1, n, cols, vocab, None, ws, size, None)
+
+    refused(L, bwd(dt=3), -1, "dy_dtype")
+    refused(L, bwd(vocab=0), -1, "bad shape")
+    refused(L, bwd(cols=0), -1, "bad shape")
+    refused(L, bwd(grad=None), -2, "grad")
+    refused(L, bwd(ld=63), -1, "ld_dy")
+    refused(L, bwd(dy=None), -1, "null")
+    refused(L, bwd(dy=PTR + 1), -2, "aligned")
+    refused(L, bwd(ws=None), -4, "workspace")
+    refused(L, bwd(size=100), -4, "workspace")
+    refused(L, bwd(ws=PTR + 4), -2, "workspace")
+    refused(L, bwd(n=(1 << 30) + 1, size=0), -1, "2^30")
+    assert bwd(n=0, dy=None, ids=None) == 0
+    size = lib.bf_embed_scaled_bwd_workspace_bytes
+    assert size(512, 64, 100) == 0 and size(513, 64, 100) > 16 * 513
+    assert size(1 << 20, 1024, 1 << 20) < 1 << 28
+
+
+def test_wrappers_refuse_before_the_library(L):
+    from bifold_amd.hip import ops
+    x = torch.zeros(4, 64)
+    q, code = torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4, 2, dtype=torch.uint8)
+    gamma, ids = torch.ones(64), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: ops.act8_pack(x), lambda: ops.act8_unpack((q, code), torch.float32),
+                 lambda: ops.act8_gelu_fwd(x, L.ACT_ERF_GELU), lambda: ops.act8_gelu_bwd(x, (q, code), L.ACT_ERF_GELU),
+                 lambda: ops.rmsnorm_fwd(x, gamma, torch.float32), lambda: ops.rmsnorm_fwd_fp8(x, gamma),
+                 lambda: ops.rmsnorm_bwd(x, x, gamma, torch.ones(4), torch.empty(64)),
+                 lambda: ops.embed_scaled_fwd(ids, x, 1.0), lambda: ops.embed_scaled_bwd(x, ids, 10, 1.0)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+    with pytest.raises(RuntimeError, match="checkpoint is"):
+        ops.act8_unpack((q, code[:, :1]), torch.float32)
+    with pytest.raises(RuntimeError, match="checkpoint is"):
+        ops.act8_unpack((q.to(torch.uint8), code), torch.float32)
+    with pytest.raises(RuntimeError, match="does not match"):
+        ops.act8_gelu_bwd(x[:3], (q, code), L.ACT_ERF_GELU)
+    buf = torch.zeros(5, 64)
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        ops.act8_gelu_bwd(buf[:4], (q, code), L.ACT_ERF_GELU, out=buf[1:])
+    with pytest.raises(RuntimeError, match="unit inner stride"):
+        ops.act8_pack(torch.zeros(64, 4).t())
+    with pytest.raises(RuntimeError, match="do not overlap"):
+        ops.act8_pack(torch.zeros(1, 64).expand(4, 64))
+    with pytest.raises(RuntimeError, match="at least one element"):
+        ops.act8_pack(torch.zeros(4, 0))
+    with pytest.raises(RuntimeError, match="gamma"):
+        ops.rmsnorm_fwd(x, gamma[:32], torch.float32)
+    with pytest.raises(RuntimeError, match="without a delta"):
+        ops.rmsnorm_fwd(x, gamma, torch.float32, x_out=torch.zeros(4, 64))
+    with pytest.raises(RuntimeError, match="x_out is x"):
+        ops.rmsnorm_fwd(buf[:4], gamma, torch.float32, delta=x, x_out=buf[1:])
+    with pytest.raises(RuntimeError, match="x_out is delta"):
+        ops.rmsnorm_fwd(x, gamma, torch.float32, delta=buf[:4], x_out=buf[1:])
+    with pytest.raises(RuntimeError, match="one shape"):
+        ops.rmsnorm_bwd(x, x[:3], gamma, torch.ones(4), torch.empty(64))
+    with pytest.raises(RuntimeError, match="out is dy"):
+        ops.rmsnorm_bwd(buf[:4], x, gamma, torch.ones(4), torch.empty(64), out=buf[1:])
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        ops.rmsnorm_bwd(x, buf[:4], gamma, torch.ones(4), torch.empty(64), out=buf[1:])
+    with pytest.raises(TypeError, match="int32"):
+        ops.embed_scaled_fwd(ids.long(), x, 1.0)
+    with pytest.raises(TypeError, match="err_flag"):
+        ops.embed_scaled_fwd(ids, x, 1.0, err_flag=torch.zeros(1))
+    with pytest.raises(RuntimeError, match="rows of dy"):
+        ops.embed_scaled_bwd(x[:3], ids, 10, 1.0)
+    with pytest.raises(ValueError, match="padding_idx"):
+        ops.embed_scaled_bwd(x, ids, 10, 1.0, padding_idx=10)
+    with pytest.raises(RuntimeError, match="add into"):
+        ops.embed_scaled_bwd(x, ids, 10, 1.0, accumulate=True)
+    with pytest.raises(RuntimeError, match="apart from dy"):
+        ops.embed_scaled_bwd(x, ids, 10, 1.0, out=torch.zeros(9, 64))
