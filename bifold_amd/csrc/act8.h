@@ -56,6 +56,32 @@ __device__ __forceinline__ void vec_store_n(T* p, int n, const float (&v)[V]) {
             if (j < n) p[j] = from_f32<T>(v[j]);
     }
 }
+// V elements as they lie in memory: nothing waits for the load until the values are taken (a conversion behind each of several
+// loads, as a branch on a run-time type or bound makes it, waits for one after the other).
+template <typename T, int V, bool AL> struct Chunk {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec r;
+    __device__ __forceinline__ void load(const void* base, size_t off, int n) {
+        const T* p = (const T*)base + off;
+        if (n >= V) {
+            constexpr int A = sizeof(vec) < 16 ? sizeof(vec) : 16;
+            if constexpr (AL) __builtin_memcpy(&r, __builtin_assume_aligned(p, A), sizeof(vec));
+            else __builtin_memcpy(&r, p, sizeof(vec));
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) r[j] = !AL && j < n ? p[j] : from_f32<T>(0.f);
+        }
+    }
+    __device__ __forceinline__ void take(float (&o)[V]) const {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = to_f32<T>(r[j]);
+    }
+    // The load is complete behind this point.  (Stores count in vmcnt too: a wait that the compiler places between stores
+    // which may or may not happen is a wait for those stores.)
+    __device__ __forceinline__ void arrived() { asm volatile("" : "+v"(r)); }
+};
+// the wave's number in its workgroup, as the scalar it is: rows, tokens and branches that depend on it stay scalar too
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 // V bytes <-> V / 4 words
 template <int V, bool AL>
 __device__ __forceinline__ void bytes_store_n(uint8_t* p, int n, const unsigned (&w)[V / 4]) {

@@ -3,8 +3,9 @@
 //   bf_embed_scaled_bwd   grad[v, :] (+)= scale * sum over { i : id_i = v } of dy[i, :]
 // The gradient is a sum over rows that share a token.  Rows are brought together by a stable radix sort of (id, i), summed in
 // runs of equal ids in the order of i, each in fp32; nothing is added with atomics, so the result is the same on every call.
-// HBM bounds both for real batches (dy read once, the table's gradient written once); the sort's few kernels are short and
-// dependent, so the zeros of a dense gradient are written by further workgroups of the same launches.
+// HBM bounds both for real batches (dy read once, the table's gradient written once).  The sort marks the tokens that occur in a
+// table of bytes, and the launch that sums the runs also writes the zeros of a dense gradient's other rows: its gathers wait for
+// latency, the zeros for bandwidth.
 #include "act8.h"
 
 namespace {
@@ -44,20 +45,20 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
     }
 }
 
-// ------------------------------------------------------------------ zeros of the dense gradient, in shares
-struct ZeroJob { float* p; size_t n; unsigned first, blocks; };            // workgroups [first, first + blocks) of the launch
-__device__ __forceinline__ void zero_share(const ZeroJob& z) {
-    const size_t at = (size_t)(blockIdx.x - z.first) * blockDim.x + threadIdx.x, step = (size_t)z.blocks * blockDim.x;
-    const size_t n4 = ((uintptr_t)z.p & 15u) == 0 ? z.n >> 2 : 0;
-    for (size_t i = at; i < n4; i += step) ((float4*)z.p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (size_t i = n4 * 4 + at; i < z.n; i += step) z.p[i] = 0.f;
+// ------------------------------------------------------------------ zeros of the dense gradient
+__global__ __launch_bounds__(512) void embed_zero_kernel(float* __restrict__ p, size_t n) {
+    const size_t at = (size_t)blockIdx.x * 512 + threadIdx.x, step = (size_t)gridDim.x * 512;
+    const size_t n4 = ((uintptr_t)p & 15u) == 0 ? n >> 2 : 0;
+    for (size_t i = at; i < n4; i += step) ((float4*)p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (size_t i = n4 * 4 + at; i < n; i += step) p[i] = 0.f;
 }
-__global__ __launch_bounds__(512) void embed_zero_kernel(const ZeroJob z) { zero_share(z); }
 
 // ------------------------------------------------------------------ the sort: least significant digit first, stable
 // A pass is two launches: counts of each digit per tile, then every tile finds its places -- for each digit the tokens of
-// smaller digits, of earlier tiles and of earlier waves -- and moves its tokens.  Digits of up to 9 bits put a vocabulary of
-// 2^18 into two passes.  Ids outside the table and the padding token become the key `vocab`, which sorts behind the others.
+// smaller digits, of earlier tiles and of earlier waves -- and moves its tokens.  (Counting the next pass's digits by global
+// atomics while moving saves a launch and costs more: 131 072 tokens 74 instead of 59 us.)  Digits of up to 9
+// bits put a vocabulary of 2^18 into two passes.  Ids outside the table and the padding token become the key `vocab`, which
+// sorts behind the others.
 #define SORT_THREADS 512
 #define SORT_WAVES 8
 #define SORT_MAX_BINS 512
@@ -65,56 +66,69 @@ __global__ __launch_bounds__(512) void embed_zero_kernel(const ZeroJob z) { zero
 
 struct SortArgs {
     const int32_t* ids; int n; int vocab; int pad;
-    const int* keys_in; const int* idx_in; int* keys_out; int* idx_out;
+    const int2* in; int2* out;                  // (key, token's place)
     int* hist; int* owner_count; int* err_flag;
+    uint8_t* present;                           // [v]: token v occurs; NULL where nobody asks
     int rounds, tiles, dbits, shift;
-    ZeroJob zero;
 };
 template <bool FIRST>
-__device__ __forceinline__ int sort_key(const SortArgs& a, int i, int* err_flag) {
+__device__ __forceinline__ int2 sort_item(const SortArgs& a, int i, int* err_flag) {
     if constexpr (FIRST) {
         const int id = a.ids[i];
         if (id < 0 || id >= a.vocab) {
             if (err_flag) atomicExch(err_flag, 1);
-            return a.vocab;
+            return make_int2(a.vocab, i);
         }
-        return id == a.pad ? a.vocab : id;
+        return make_int2(id == a.pad ? a.vocab : id, i);
     } else {
-        return a.keys_in[i];
+        return a.in[i];
     }
 }
 template <bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void embed_hist_kernel(const SortArgs a) {
     __shared__ int bins[SORT_MAX_BINS];
-    if ((int)blockIdx.x >= a.tiles) { zero_share(a.zero); return; }
     if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) *a.owner_count = 0;
+    if (FIRST && a.present) {
+        unsigned* words = (unsigned*)a.present;
+        const int many = (int)(((unsigned)a.vocab + 3u) >> 2);
+        for (int i = blockIdx.x * SORT_THREADS + threadIdx.x; i < many; i += a.tiles * SORT_THREADS) words[i] = 0;
+    }
     bins[threadIdx.x] = 0;
     __syncthreads();
-    const int span = SORT_THREADS * a.rounds, base = blockIdx.x * span, mask = (1 << a.dbits) - 1;
+    const int base = blockIdx.x * SORT_THREADS * a.rounds, mask = (1 << a.dbits) - 1;
     for (int r = 0; r < a.rounds; ++r) {
         const int i = base + r * SORT_THREADS + threadIdx.x;
-        if (i < a.n) atomicAdd(&bins[(sort_key<FIRST>(a, i, a.err_flag) >> a.shift) & mask], 1);
+        if (i < a.n) atomicAdd(&bins[(sort_item<FIRST>(a, i, a.err_flag).x >> a.shift) & mask], 1);
     }
     __syncthreads();
-    if ((int)threadIdx.x <= mask) a.hist[blockIdx.x * SORT_MAX_BINS + threadIdx.x] = bins[threadIdx.x];
+    a.hist[blockIdx.x * SORT_MAX_BINS + threadIdx.x] = bins[threadIdx.x];
 }
 template <bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortArgs a) {
     __shared__ int cnt[SORT_WAVES][SORT_MAX_BINS];
     __shared__ int wave_tot[SORT_WAVES];
-    if ((int)blockIdx.x >= a.tiles) { zero_share(a.zero); return; }
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int mask = (1 << a.dbits) - 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int mask = (1 << a.dbits) - 1, span = SORT_THREADS * a.rounds;
 #pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) cnt[w][tid] = 0;
-    // all tokens of this digit, and those in earlier tiles
+    __syncthreads();
+    // a wave owns `rounds` x 64 consecutive tokens of the tile
+    const int first = blockIdx.x * span + wave * 64 * a.rounds + lane;
+#pragma unroll 4
+    for (int r = 0; r < a.rounds; ++r) {
+        const int i = first + r * 64;
+        if (i < a.n) atomicAdd(&cnt[wave][(sort_item<FIRST>(a, i, nullptr).x >> a.shift) & mask], 1);
+    }
+    // all tokens of this thread's digit, and those in earlier tiles: sixteen tiles' counts in flight
     int tot = 0, before = 0;
-    if (tid <= mask) {
-#pragma unroll 8
-        for (int t = 0; t < a.tiles; ++t) {
-            const int h = a.hist[t * SORT_MAX_BINS + tid];
-            tot += h;
-            before += t < (int)blockIdx.x ? h : 0;
+    for (int t0 = 0; t0 < a.tiles; t0 += 16) {
+        int h[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) h[u] = a.hist[min(t0 + u, a.tiles - 1) * SORT_MAX_BINS + tid];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            tot += t0 + u < a.tiles ? h[u] : 0;
+            before += t0 + u < (int)blockIdx.x ? h[u] : 0;
         }
     }
     int scan = tot;                             // inclusive over the digits
@@ -127,13 +141,7 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
     __syncthreads();
     for (int w = 0; w < wave; ++w) scan += wave_tot[w];
     int place = scan - tot + before;
-    // a wave owns `rounds` x 64 consecutive tokens of the tile
-    const int first = blockIdx.x * SORT_THREADS * a.rounds + wave * 64 * a.rounds + lane;
-    for (int r = 0; r < a.rounds; ++r) {
-        const int i = first + r * 64;
-        if (i < a.n) atomicAdd(&cnt[wave][(sort_key<FIRST>(a, i, nullptr) >> a.shift) & mask], 1);
-    }
-    __syncthreads();
+#pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) {
         const int c = cnt[w][tid];
         cnt[w][tid] = place;
@@ -144,10 +152,13 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
     // by a ballot per digit bit; the first of them moves the place on.  LDS accesses of one wave complete in order; the
     // relaxed atomics keep the compiler from holding a place in a register.
     int* mine = cnt[wave];
+    int2 item = first < a.n ? sort_item<FIRST>(a, first, nullptr) : make_int2(0, 0);
     for (int r = 0; r < a.rounds; ++r) {
         const int i = first + r * 64;
         const bool live = i < a.n;
-        const int key = live ? sort_key<FIRST>(a, i, nullptr) : 0, d = (key >> a.shift) & mask;
+        const int2 it = item;
+        if (r + 1 < a.rounds && i + 64 < a.n) item = sort_item<FIRST>(a, i + 64, nullptr);
+        const int d = (it.x >> a.shift) & mask;
         unsigned long long same = __ballot(live);
         for (int b = 0; b < a.dbits; ++b) {
             const bool bit = (d >> b) & 1;
@@ -157,18 +168,19 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
         const int rank = __popcll(same & ((1ull << lane) - 1ull));
         if (live) {
             const int at = __hip_atomic_load(&mine[d], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-            a.keys_out[at + rank] = key;
-            a.idx_out[at + rank] = FIRST ? i : a.idx_in[i];
+            a.out[at + rank] = it;
             if (rank == 0) __hip_atomic_store(&mine[d], at + __popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            if (FIRST && a.present && it.x < a.vocab) a.present[it.x] = 1;     // whoever stores it, it is the same byte
         }
     }
 }
 
 // ------------------------------------------------------------------ sums over runs of equal keys
 struct SumArgs {
-    const int* keys; const int* idx; int n; int vocab; int chunk, chunks, slabs;
+    const int2* sorted; int n; int vocab; int chunk, chunks, slabs;        // (key, row of dy), by key, then row
     const void* dy; int64_t ld; int cols; float scale; int accumulate;
-    float* grad; float* part; int* owners; int* owner_count;
+    float* grad; float* part; int2* owners; int* owner_count;              // owners: (chunk, key) of each cut run
+    const uint8_t* present; unsigned sum_blocks;                 // present: NULL, or the other rows' zeros are written too
 };
 template <int V, bool AL>
 __device__ __forceinline__ void grad_write(const SumArgs& a, int key, int c, const float (&acc)[V]) {
@@ -179,85 +191,139 @@ __device__ __forceinline__ void grad_write(const SumArgs& a, int key, int c, con
     for (int j = 0; j < V; ++j) o[j] = a.accumulate ? o[j] + acc[j] * a.scale : acc[j] * a.scale;
     vec_store_n<float, V, AL>(g, a.cols - c, o);
 }
-// One wave takes `chunk` (at most 64) consecutive sorted tokens and 64 V columns, eight rows in flight.  A run that lies
-// inside the chunk goes to the gradient; the sum of a run that reaches over an end goes to part[chunk][0] (it began in an
-// earlier chunk) or part[chunk][1] (it begins here: this chunk owns the run and is noted for embed_join_kernel).
+// One wave takes `chunk` (at most 64) consecutive sorted tokens and 64 V columns, eight rows in flight.  A run of equal keys
+// belongs to the chunk it begins in, which follows it into the next chunk.  Only a run that covers a whole further chunk is
+// cut: its sum over the chunk it begins in goes to part[chunk][1] (that chunk owns the run and notes it for
+// embed_join_kernel), its sums over the chunks it reaches into go to part[.][0].
 template <typename T, int V, bool AL>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
     const int lane = threadIdx.x & 63;
-    const unsigned w = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (blockIdx.x >= a.sum_blocks) {           // a wave per eight rows of the table
+        const size_t group = (size_t)(blockIdx.x - a.sum_blocks) * 4 + wave_id(), row0 = group * 8;
+        if (row0 >= (size_t)a.vocab) return;
+        const int rows = (int)min((size_t)8, a.vocab - row0);
+        const unsigned long long there = __ballot(lane >= rows || a.present[row0 + (lane & 7)] != 0);
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < rows; ++r) {
+            if ((there >> r) & 1) continue;
+            float* g = a.grad + (row0 + r) * a.cols;
+            for (int c = lane * 4; c < a.cols; c += 256) vec_store_n<float, 4, AL>(g + c, a.cols - c, zero);
+        }
+        return;
+    }
+    const unsigned w = blockIdx.x * 4u + (unsigned)wave_id();
     const int chunk = (int)(w / (unsigned)a.slabs), slab = (int)(w - (unsigned)chunk * (unsigned)a.slabs);
     if (chunk >= a.chunks) return;
     const int s = chunk * a.chunk, here = min(a.chunk, a.n - s);
-    const int kl = lane < here ? a.keys[s + lane] : a.vocab;
-    const int il = lane < here ? a.idx[s + lane] : 0;
-    const int prev = s > 0 ? a.keys[s - 1] : -1, next = s + here < a.n ? a.keys[s + here] : -1;
+    const int there = max(0, min(a.chunk, a.n - s - a.chunk));            // tokens of the next chunk
+    const int2 mine = lane < here ? a.sorted[s + lane] : make_int2(a.vocab, 0);
+    const int2 ahead = lane < there ? a.sorted[s + a.chunk + lane] : make_int2(-1, 0);
+    const int kl = mine.x, il = mine.y, kn = ahead.x, in = ahead.y;
+    // uniform addresses: scalar loads
+    const int prev = s > 0 ? a.sorted[s - 1].x : -1, prev2 = s > a.chunk ? a.sorted[s - a.chunk - 1].x : -1;
+    const int next2 = s + 2 * a.chunk < a.n ? a.sorted[s + 2 * a.chunk].x : -1;
     const int live = __popcll(__ballot(lane < here && kl < a.vocab));      // sorted: the live ones come first
+    if (live == 0) return;
     const int c = (slab * 64 + lane) * V, nc = a.cols - c;
-    const T* dy = (const T*)a.dy + c;
     float* part = a.part + (size_t)chunk * 2 * a.cols + c;
+    const int k_first = __builtin_amdgcn_readlane(kl, 0), k_last = __builtin_amdgcn_readlane(kl, live - 1);
+    const int next = there > 0 ? __builtin_amdgcn_readfirstlane(kn) : -1;
+    // the run this chunk begins inside of: the chunk before has it if it began there and ends here
+    bool head = k_first == prev;
+    int i = 0;
+    if (head && prev2 != k_first && next != k_first) {
+        i = __popcll(__ballot(lane < here && kl == k_first));
+        head = false;
+    }
+    // the run this chunk ends inside of: followed to its end if that lies in the next chunk
+    const bool open = live == here && next == k_last, cut = open && next2 == k_last;
+    const bool whole = head && k_first == k_last;                          // began before and fills the chunk
+    int stop = live;
+    if (open && !cut && !whole) stop += __popcll(__ballot(lane < there && kn == k_last));
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
-    bool head = live > 0 && __builtin_amdgcn_readlane(kl, 0) == prev;
-    for (int i0 = 0; i0 < live; i0 += 8) {
-        float f[8][V];
+    while (i < stop) {
+        Chunk<T, V, AL> f[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            if (i0 + u < live) {
-                const int row = __builtin_amdgcn_readlane(il, i0 + u);
-                vec_load_n<T, V, AL>(dy + (size_t)row * a.ld, nc, f[u]);
-            }
+            const int at = min(i + u, stop - 1);
+            const int row = at < here ? __builtin_amdgcn_readlane(il, at) : __builtin_amdgcn_readlane(in, at - here);
+            f[u].load(a.dy, (size_t)row * a.ld + c, nc);
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = i0 + u;
-            if (i < live) {
+        for (int u = 0; u < 8; ++u) f[u].arrived();
 #pragma unroll
-                for (int j = 0; j < V; ++j) acc[j] += f[u][j];
-                const int key = __builtin_amdgcn_readlane(kl, i);
-                const bool last = i + 1 == here;
-                const int after = last ? next : __builtin_amdgcn_readlane(kl, i + 1);
+        for (int u = 0; u < 8; ++u) {
+            if (i + u < stop) {
+                const int at = i + u;
+                float v[V];
+                f[u].take(v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[j] += v[j];
+                const int key = at < here ? __builtin_amdgcn_readlane(kl, at) : k_last;
+                // the key behind this token; a cut run ends with the chunk
+                const int after = at + 1 == stop ? -1 : at + 1 < here ? __builtin_amdgcn_readlane(kl, at + 1) : k_last;
                 if (after != key) {
-                    if (head) vec_store_n<float, V, AL>(part, nc, acc);
-                    else grad_write<V, AL>(a, key, c, acc);
+                    if (head) {
+                        vec_store_n<float, V, AL>(part, nc, acc);
+                    } else if (cut && at + 1 == stop) {
+                        vec_store_n<float, V, AL>(part + a.cols, nc, acc);
+                        if (slab == 0 && lane == 0) a.owners[atomicAdd(a.owner_count, 1)] = make_int2(chunk, key);
+                    } else {
+                        grad_write<V, AL>(a, key, c, acc);
+                    }
                     head = false;
 #pragma unroll
                     for (int j = 0; j < V; ++j) acc[j] = 0.f;
-                } else if (last) {
-                    vec_store_n<float, V, AL>(head ? part : part + a.cols, nc, acc);
-                    if (!head && slab == 0 && lane == 0) a.owners[atomicAdd(a.owner_count, 1)] = chunk;
                 }
             }
         }
+        i += 8;
     }
 }
-// One workgroup per owned run (their order in the list does not matter: each has a gradient row of its own) and 256 columns:
+// One workgroup per cut run (their order in the list does not matter: each has a gradient row of its own) and 256 columns:
 // finds the last chunk that starts with the run's key, sums the partial rows in order, sixteen waves a share each.
 __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
     __shared__ float4 red[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ int found[16];
+    const int lane = threadIdx.x & 63, wave = wave_id();
     const int slabs = (a.cols + 255) / 256;
     const int total = *a.owner_count * slabs;
     for (int wk = blockIdx.x; wk < total; wk += gridDim.x) {
-        const int chunk = a.owners[wk / slabs], c = (wk % slabs) * 256 + lane * 4, nc = a.cols - c;
-        const int key = a.keys[(size_t)(chunk + 1) * a.chunk - 1];
+        const int2 owner = a.owners[wk / slabs];
+        const int chunk = owner.x, key = owner.y, c = (wk % slabs) * 256 + lane * 4, nc = a.cols - c;
         int lo = chunk + 1, hi = a.chunks;      // chunk lo starts with the key; hi does not (or is behind the last)
-        while (hi - lo > 1) {
-            const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
-            const bool in = at < hi && a.keys[(size_t)at * a.chunk] == key;
-            lo += step * __popcll(__ballot(in));
+        while (hi - lo > 1) {                   // 1 024 places at a time
+            const int step = (hi - lo + 1023) >> 10, at = lo + ((int)threadIdx.x + 1) * step;
+            const bool in = at < hi && a.sorted[(size_t)at * a.chunk].x == key;
+            const int votes = __popcll(__ballot(in));
+            if (lane == 0) found[wave] = votes;
+            __syncthreads();
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sum += found[k];
+            lo += step * sum;
             hi = min(hi, lo + step);
+            __syncthreads();
         }
         const int many = lo - chunk + 1, share = (many + 15) >> 4;          // partial rows: part[chunk][1], part[chunk + 1 ..][0]
         const int from = wave * share, to = min(many, from + share);
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int t = from; t < to; ++t) {
-            float f[4];
-            vec_load_n<float, 4, false>(a.part + ((size_t)(chunk + t) * 2 + (t == 0)) * a.cols + c, nc, f);
+        for (int t = from; t < to; t += 8) {
+            Chunk<float, 4, false> f[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] += f[j];
+            for (int u = 0; u < 8; ++u) {
+                const int at = min(t + u, to - 1);
+                f[u].load(a.part, ((size_t)(chunk + at) * 2 + (at == 0)) * a.cols + c, nc);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                float v[4];
+                f[u].take(v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] += t + u < to ? v[j] : 0.f;
+            }
         }
         red[wave][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         __syncthreads();
@@ -283,7 +349,7 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
     __shared__ unsigned long long words[FEW / 64];
     __shared__ unsigned short list[FEW];
     __shared__ float red[FEW / 64][64 * V];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, me = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), me = blockIdx.x;
     const int key = ids[me];
     if (key < 0 || key >= a.vocab) {
         if (tid == 0 && err_flag) atomicExch(err_flag, 1);
@@ -317,12 +383,17 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
         float acc[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = 0.f;
-#pragma unroll 4
-        for (int t = from; t < to; ++t) {
-            float f[V];
-            vec_load_n<T, V, AL>((const T*)a.dy + (size_t)list[t] * a.ld + c, nc, f);
+        for (int t = from; t < to; t += 4) {
+            Chunk<T, V, AL> f[4];
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += f[j];
+            for (int u = 0; u < 4; ++u) f[u].load(a.dy, (size_t)list[min(t + u, to - 1)] * a.ld + c, nc);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float v[V];
+                f[u].take(v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[j] += t + u < to ? v[j] : 0.f;
+            }
         }
         if (shares > 1) {
 #pragma unroll
@@ -342,7 +413,7 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
 // ------------------------------------------------------------------ plan of a call
 struct EmbedPlan {
     int passes, dbits, rounds, tiles, chunk, chunks;
-    size_t keys, hist, owners, part, bytes;     // offsets into the workspace
+    size_t pairs, hist, owners, present, part, bytes;            // offsets into the workspace
 };
 EmbedPlan embed_plan(int n, int cols, int vocab) {
     EmbedPlan p;
@@ -353,22 +424,25 @@ EmbedPlan embed_plan(int n, int cols, int vocab) {
     const long span = (long)SORT_THREADS * SORT_MAX_TILES;
     p.rounds = (int)((n + span - 1) / span);
     p.tiles = (n + SORT_THREADS * p.rounds - 1) / (SORT_THREADS * p.rounds);
-    // tokens per wave: enough waves for the chip first, then few partial rows
-    p.chunk = n >= 65536 ? 64 : n >= 16384 ? 32 : 16;
+    // tokens per wave: enough waves for the chip first, then few partial rows (131 072 tokens x 1 024: sum + join 108.9 us with
+    // 64, 102.6 with 32; 8 192 x 768: 25.2 us with 16, 26.8 with 8)
+    p.chunk = n >= 16384 ? 32 : 16;
     p.chunks = (n + p.chunk - 1) / p.chunk;
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    p.keys = 0;
+    p.pairs = 0;
     p.hist = up((size_t)n * 16);
     p.owners = p.hist + up((size_t)p.tiles * SORT_MAX_BINS * 4);
-    p.part = p.owners + up((size_t)(p.chunks + 1) * 4);
+    p.present = p.owners + up((size_t)(p.chunks + 1) * 8);
+    p.part = p.present + up((size_t)vocab + 8);
     p.bytes = p.part + up((size_t)p.chunks * 2 * cols * 4);
     return p;
 }
 
 template <typename T, int V, bool AL>
-void embed_sum_launch(const SumArgs& a, hipStream_t s) {
-    const size_t waves = (size_t)a.chunks * a.slabs;
-    hipLaunchKernelGGL((embed_sum_kernel<T, V, AL>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a);
+void embed_sum_launch(SumArgs a, hipStream_t s) {
+    a.sum_blocks = (unsigned)(((size_t)a.chunks * a.slabs + 3) / 4);
+    const unsigned zeros = a.present ? (unsigned)(((size_t)a.vocab + 31) / 32) : 0u;
+    hipLaunchKernelGGL((embed_sum_kernel<T, V, AL>), dim3(a.sum_blocks + zeros), dim3(256), 0, s, a);
 }
 template <typename T, int V>
 void embed_bwd_type(bool few, bool al, const int32_t* ids, int pad, int* err_flag, const SumArgs& a, hipStream_t s) {
@@ -433,21 +507,12 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
     BF_REQUIRE(n <= (1 << 30), BF_EINVAL, "%s: over 2^30 tokens (n=%d)", name, n);
     BF_REQUIRE(grad && (uintptr_t)grad % 4 == 0, BF_EALIGN, "%s: grad is null or not aligned to its element", name);
     hipStream_t s = (hipStream_t)stream;
-    const size_t floats = accumulate ? 0 : (size_t)vocab * cols;
-    auto zero_job = [&](size_t from, size_t to, unsigned first) {
-        ZeroJob z = {grad + from, to - from, first, 0};
-        size_t b = (z.n + 8191) / 8192;                          // four 16-byte stores per thread, more for large tables
-        z.blocks = (unsigned)(b < 2048 ? b : 2048);
-        return z;
-    };
-    if (n <= FEW) {
-        const ZeroJob z = zero_job(0, floats, 0);
-        if (z.blocks) {
-            hipLaunchKernelGGL(embed_zero_kernel, dim3(z.blocks), dim3(512), 0, s, z);
-            BF_CHECK_LAUNCH(name);
-        }
-        if (n == 0) return BF_OK;
+    if (n <= FEW && !accumulate) {
+        const size_t floats = (size_t)vocab * cols, blocks = (floats + 8191) / 8192;             // four 16-byte stores per thread
+        hipLaunchKernelGGL(embed_zero_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(512), 0, s, grad, floats);
+        BF_CHECK_LAUNCH(name);
     }
+    if (n == 0) return BF_OK;
     BF_REQUIRE(dy && tokens, BF_EINVAL, "%s: null pointer", name);
     BF_REQUIRE(ld_dy >= cols, BF_EINVAL, "%s: ld_dy=%lld is under cols=%d", name, (long long)ld_dy, cols);
     const size_t esz = bf_dtype_size(dy_dtype);
@@ -465,33 +530,29 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
                    workspace_bytes, p.bytes);
         BF_REQUIRE(bf_aligned16(workspace), BF_EALIGN, "%s: unaligned workspace", name);
         char* ws = (char*)workspace;
-        int* buf[4];
-        for (int k = 0; k < 4; ++k) buf[k] = (int*)(ws + p.keys) + (size_t)k * n;
-        int* owners = (int*)(ws + p.owners);
+        int2* const pairs[2] = {(int2*)(ws + p.pairs), (int2*)(ws + p.pairs) + n};
+        int2* owners = (int2*)(ws + p.owners);
         SortArgs q = {};
         q.ids = tokens; q.n = n; q.vocab = vocab; q.pad = padding_idx; q.hist = (int*)(ws + p.hist);
-        q.owner_count = owners + p.chunks; q.err_flag = err_flag; q.rounds = p.rounds; q.tiles = p.tiles; q.dbits = p.dbits;
-        const int launches = 2 * p.passes;
-        size_t done = 0;
+        q.owner_count = (int*)(owners + p.chunks); q.err_flag = err_flag; q.rounds = p.rounds; q.tiles = p.tiles; q.dbits = p.dbits;
+        q.present = accumulate ? nullptr : (uint8_t*)(ws + p.present);
+        const dim3 grid((unsigned)p.tiles), block(SORT_THREADS);
         for (int pass = 0; pass < p.passes; ++pass) {
             q.shift = pass * p.dbits;
-            q.keys_in = buf[2 * ((pass + 1) & 1)]; q.idx_in = buf[2 * ((pass + 1) & 1) + 1];
-            q.keys_out = buf[2 * (pass & 1)]; q.idx_out = buf[2 * (pass & 1) + 1];
-            for (int half = 0; half < 2; ++half) {
-                const int k = 2 * pass + half + 1;
-                const size_t to = k == launches ? floats : floats / launches * k & ~(size_t)3;
-                q.zero = zero_job(done, to, (unsigned)p.tiles);
-                done = to;
-                const dim3 grid((unsigned)p.tiles + q.zero.blocks), block(SORT_THREADS);
-                if (half == 0 && pass == 0) hipLaunchKernelGGL((embed_hist_kernel<true>), grid, block, 0, s, q);
-                else if (half == 0) hipLaunchKernelGGL((embed_hist_kernel<false>), grid, block, 0, s, q);
-                else if (pass == 0) hipLaunchKernelGGL((embed_scatter_kernel<true>), grid, block, 0, s, q);
-                else hipLaunchKernelGGL((embed_scatter_kernel<false>), grid, block, 0, s, q);
-                BF_CHECK_LAUNCH(name);
+            q.in = pairs[(pass + 1) & 1];
+            q.out = pairs[pass & 1];
+            if (pass == 0) {
+                hipLaunchKernelGGL((embed_hist_kernel<true>), grid, block, 0, s, q);
+                hipLaunchKernelGGL((embed_scatter_kernel<true>), grid, block, 0, s, q);
+            } else {
+                hipLaunchKernelGGL((embed_hist_kernel<false>), grid, block, 0, s, q);
+                hipLaunchKernelGGL((embed_scatter_kernel<false>), grid, block, 0, s, q);
             }
+            BF_CHECK_LAUNCH(name);
         }
-        a.keys = q.keys_out; a.idx = q.idx_out; a.chunk = p.chunk; a.chunks = p.chunks;
-        a.part = (float*)(ws + p.part); a.owners = owners; a.owner_count = owners + p.chunks;
+        a.present = q.present;
+        a.sorted = q.out; a.chunk = p.chunk; a.chunks = p.chunks; a.owners = owners; a.owner_count = q.owner_count;
+        a.part = (float*)(ws + p.part);
     }
     if (dy_dtype == BF_F32) embed_bwd_type<float, 4>(few, al, tokens, padding_idx, err_flag, a, s);
     else if (dy_dtype == BF_BF16) embed_bwd_type<bf16_t, 8>(few, al, tokens, padding_idx, err_flag, a, s);

@@ -101,13 +101,28 @@ __device__ __forceinline__ void keep8(const RmsFwd& a, int row, int c, int n, co
     if ((c & 31) == 0 && n > 0) a.code[(size_t)row * a.gpr + (c >> 5)] = (uint8_t)code;
 }
 
+template <typename TD, int V, int T, int NV, bool AL>
+__device__ __forceinline__ void add_row(const RmsFwd& a, int row, int slot, float (&t)[NV][V]) {
+    const TD* p = (const TD*)a.delta + (size_t)row * a.ldd;
+    float d[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * T + slot) * V;
+        vec_load_n<TD, V, AL>(p + c, a.cols - c, d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[i][j] += d[i][j];
+}
+
 // ------------------------------------------------------------------ forward, the row in registers (cols <= 64 WPR V NV)
 template <typename TX, int V, int WPR, int NV, bool AL>
 __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
     constexpr int T = 64 * WPR;
     __shared__ float red_s[4];
     __shared__ unsigned red_m[4];
-    const int row = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int row = WPR == 1 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
     if (row >= a.rows) return;
     const int slot = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
     const TX* x = (const TX*)a.x + (size_t)row * a.ldx;
@@ -117,17 +132,10 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
         const int c = (i * T + slot) * V;
         vec_load_n<TX, V, AL>(x + c, a.cols - c, t[i]);
     }
-    if (a.delta) {
-        float d[NV][V];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * T + slot) * V;
-            load_as<V, AL>(a.delta, a.d_dtype, (size_t)row * a.ldd + c, a.cols - c, d[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) t[i][j] += d[i][j];
+    if (a.delta) {                              // all chunks' loads first: a conversion between them would wait for each
+        if (a.d_dtype == BF_F32) add_row<float, V, T, NV, AL>(a, row, slot, t);
+        else if (a.d_dtype == BF_BF16) add_row<bf16_t, V, T, NV, AL>(a, row, slot, t);
+        else add_row<f16_t, V, T, NV, AL>(a, row, slot, t);
     }
     float s = 0.f;
 #pragma unroll
@@ -245,31 +253,38 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
 }
 
 // ------------------------------------------------------------------ backward
-// t of one chunk: from the tensor, or from the checkpoint
-template <int V, bool AL>
-__device__ __forceinline__ void stream_load(const RmsBwd& a, int row, int c, int n, float (&t)[V]) {
-    if (a.q) {
-        unsigned w[V / 4];
+struct Kept {};                                 // the stream is a checkpoint
+
+template <typename TX, int V, bool AL> struct StreamChunk {
+    Chunk<TX, V, AL> x;
+    __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) { x.load(a.x, (size_t)row * a.ldx + c, n); }
+    __device__ __forceinline__ void take(int, float (&t)[V]) const { x.take(t); }
+};
+template <int V, bool AL> struct StreamChunk<Kept, V, AL> {
+    unsigned w[V / 4], code;
+    __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) {
         bytes_load_n<V, AL>(a.q + (size_t)row * a.cols + c, n, w);
-        const unsigned code = n > 0 ? a.code[(size_t)row * a.gpr + (c >> 5)] : 1u;
+        code = n > 0 ? a.code[(size_t)row * a.gpr + (c >> 5)] : 1u;
+    }
+    __device__ __forceinline__ void take(int n, float (&t)[V]) const {
         act8_dequant<V>(w, code, t);
-        if (n < V) {
+        if (!AL && n < V) {                     // a NaN group's missing columns are no part of the row
 #pragma unroll
             for (int j = 0; j < V; ++j) t[j] = j < n ? t[j] : 0.f;
         }
-    } else {
-        load_as<V, AL>(a.x, a.x_dtype, (size_t)row * a.ldx + c, n, t);
     }
-}
+};
 
 // Workgroups walk rows (nblk of them side by side); a lane keeps its columns' share of dgamma over all its rows in
-// registers, the workgroup writes one row of partial sums and rms_dgamma_kernel adds those in a fixed order.
-template <typename TDY, int V, int WPR, int NV, bool AL>
+// registers, the workgroup writes one row of partial sums and rms_dgamma_kernel adds those in a fixed order.  A row's three
+// loads are issued together, in the types they have (template: a branch on a type at run time would convert, and so wait,
+// between them).
+template <typename TDY, typename TX, typename TD, int V, int WPR, int NV, bool AL>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
     constexpr int T = 64 * WPR;
     __shared__ float red[2][4];
     extern __shared__ float fold[];             // WPR == 1: [4][cols]
-    const int wave = threadIdx.x >> 6;
+    const int wave = wave_id();
     const int slot = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
     const int stride = WPR == 1 ? a.nblk * 4 : a.nblk;
     float g[NV][V], acc[NV][V];
@@ -282,22 +297,28 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
     }
     int turn = 0;
     for (int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x; row < a.rows; row += stride, turn ^= 1) {
-        const TDY* dy = (const TDY*)a.dy + (size_t)row * a.ldy;
-        float b[NV][V], h[NV][V];
+        Chunk<TDY, V, AL> dy[NV];
+        StreamChunk<TX, V, AL> x[NV];
+        Chunk<TD, V, AL> dres[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
-            vec_load_n<TDY, V, AL>(dy + c, a.cols - c, b[i]);
+            dy[i].load(a.dy, (size_t)row * a.ldy + c, a.cols - c);
+            x[i].load(a, row, c, a.cols - c);
         }
+        if (a.dres) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * T + slot) * V;
-            stream_load<V, AL>(a, row, c, a.cols - c, h[i]);
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * T + slot) * V;
+                dres[i].load(a.dres, (size_t)row * a.ldr + c, a.cols - c);
+            }
         }
         const float r = a.rstd[row];
-        float s = 0.f;
+        float b[NV][V], h[NV][V], s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            dy[i].take(b[i]);
+            x[i].take(a.cols - (i * T + slot) * V, h[i]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 h[i][j] *= r;
@@ -305,20 +326,20 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
                 b[i][j] *= g[i][j];
                 s = fmaf(b[i][j], h[i][j], s);
             }
+        }
         const float m = row_sum<WPR>(s, red[turn]) / (float)a.cols;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V, n = a.cols - c;
-            float o[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) o[j] = r * (b[i][j] - h[i][j] * m);
+            for (int j = 0; j < V; ++j) b[i][j] = r * (b[i][j] - h[i][j] * m);
             if (a.dres) {
                 float d[V];
-                load_as<V, AL>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, n, d);
+                dres[i].take(d);
 #pragma unroll
-                for (int j = 0; j < V; ++j) o[j] += d[j];
+                for (int j = 0; j < V; ++j) b[i][j] += d[j];
             }
-            store_as<V, AL>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, n, o);
+            vec_store_n<TD, V, AL>((TD*)a.dx + (size_t)row * a.cols + c, n, b[i]);
         }
     }
     float* part = a.part + (size_t)blockIdx.x * a.cols;
@@ -342,7 +363,20 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
     }
 }
 
-// any width: dx by one workgroup per row, two walks; dgamma by columns, a thread per column and chunk of rows
+// t of one chunk, its type chosen at run time
+template <int V>
+__device__ __forceinline__ void stream_load(const RmsBwd& a, int row, int c, int n, float (&t)[V]) {
+    if (a.q) {
+        StreamChunk<Kept, V, false> k;
+        k.load(a, row, c, n);
+        k.take(n, t);
+    } else {
+        load_as<V, false>(a.x, a.x_dtype, (size_t)row * a.ldx + c, n, t);
+    }
+}
+
+// any width and any mixture of types: dx by one workgroup per row, two walks; dgamma by columns, a thread per column and
+// chunk of rows
 template <typename TDY>
 __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
     constexpr int V = 8;
@@ -354,7 +388,7 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
         float g[V];
         vec_load_n<TDY, V, false>(dy + c, a.cols - c, b);
         vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
-        stream_load<V, false>(a, row, c, a.cols - c, h);
+        stream_load<V>(a, row, c, a.cols - c, h);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             b[j] *= g[j];
@@ -381,8 +415,7 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
         store_as<V, false>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, a.cols - c, b);
     }
 }
-// Every dy and t it reads was read by rms_bwd_long_kernel too; dx must therefore not overwrite dy (the entry point refuses
-// dx == dy for these widths).
+// Launched in front of rms_bwd_long_kernel, which may write dx over dy.
 template <typename TDY>
 __global__ __launch_bounds__(256) void rms_dgamma_long_kernel(const RmsBwd a) {
     const int c = blockIdx.x * 256 + threadIdx.x;
@@ -446,11 +479,11 @@ template <typename TX, int V, bool AL> void rms_fwd_launch(const RmsFwd& a, hipS
     }
 #undef RMS_FWD
 }
-template <typename TDY, int V, bool AL> void rms_bwd_launch(const RmsBwd& a, hipStream_t s) {
+template <typename TDY, typename TX, typename TD, int V, bool AL> void rms_bwd_launch(const RmsBwd& a, hipStream_t s) {
     const dim3 grid((unsigned)a.nblk), block(256);
     const int chunks = (a.cols + V - 1) / V;
     const size_t lds = (size_t)16 * a.cols;     // WPR == 1: at most 16 KB
-#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, V, W, N, AL>), grid, block, W == 1 ? lds : 0, s, a)
+#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, TX, TD, V, W, N, AL>), grid, block, W == 1 ? lds : 0, s, a)
     if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
         if (chunks <= 64) RMS_BWD(1, 1);
         else if (chunks <= 128) RMS_BWD(1, 2);
@@ -475,15 +508,31 @@ template <typename TX> void rms_fwd_any(const RmsFwd& a, bool al, hipStream_t s)
     else if (al) rms_fwd_launch<TX, V, true>(a, s);
     else rms_fwd_launch<TX, V, false>(a, s);
 }
-template <typename TDY> void rms_bwd_any(const RmsBwd& a, bool al, hipStream_t s) {
+template <typename TDY, typename TX, typename TD> void rms_bwd_types(const RmsBwd& a, bool al, hipStream_t s) {
     constexpr int V = sizeof(TDY) == 4 ? 4 : 8;
-    if (a.cols > RMS_LONG) {
+    if (al) rms_bwd_launch<TDY, TX, TD, V, true>(a, s);
+    else rms_bwd_launch<TDY, TX, TD, V, false>(a, s);
+}
+// dy, x and dx of one 16-bit type or fp32, with dy fp32 only beside fp32: what training steps have.  Wider rows and other
+// mixtures take the kernels that walk.
+template <typename TDY> constexpr int dtype_of() { return sizeof(TDY) == 4 ? BF_F32 : __is_same(TDY, bf16_t) ? BF_BF16 : BF_F16; }
+bool rms_bwd_walks(int dy_dtype, int x_dtype, bool kept, int dx_dtype, int cols) {
+    const bool x_ok = kept || x_dtype == BF_F32 || x_dtype == dy_dtype, d_ok = dx_dtype == BF_F32 || dx_dtype == dy_dtype;
+    return cols > RMS_LONG || !x_ok || !d_ok;
+}
+template <typename TDY> void rms_bwd_any(const RmsBwd& a, bool al, hipStream_t s) {
+    constexpr int dt = dtype_of<TDY>();
+    if (rms_bwd_walks(dt, a.x_dtype, a.q != nullptr, a.dx_dtype, a.cols)) {
         hipLaunchKernelGGL((rms_dgamma_long_kernel<TDY>), dim3((unsigned)((a.cols + 255) / 256), (unsigned)a.nblk), dim3(256), 0, s, a);
         hipLaunchKernelGGL((rms_bwd_long_kernel<TDY>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
-    } else if (al) {
-        rms_bwd_launch<TDY, V, true>(a, s);
+    } else if (a.dx_dtype == dt) {
+        if (a.q) rms_bwd_types<TDY, Kept, TDY>(a, al, s);
+        else if (a.x_dtype == dt) rms_bwd_types<TDY, TDY, TDY>(a, al, s);
+        else rms_bwd_types<TDY, float, TDY>(a, al, s);
     } else {
-        rms_bwd_launch<TDY, V, false>(a, s);
+        if (a.q) rms_bwd_types<TDY, Kept, float>(a, al, s);
+        else if (a.x_dtype == dt) rms_bwd_types<TDY, TDY, float>(a, al, s);
+        else rms_bwd_types<TDY, float, float>(a, al, s);
     }
 }
 
@@ -568,7 +617,6 @@ extern "C" int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const
     BF_REQUIRE(dy && gamma && rstd && dx && parts_ws, BF_EINVAL, "%s: null pointer", name);
     BF_REQUIRE(ld_dy >= cols && (!x || ldx >= cols) && (!dres || ld_dres >= cols), BF_EINVAL,
                "%s: a leading dimension is under cols=%d", name, cols);
-    BF_REQUIRE(cols <= RMS_LONG || dx != dy, BF_EINVAL, "%s: dx may be dy up to %d columns only", name, RMS_LONG);
     BF_REQUIRE(dx != dy || (ld_dy == cols && dx_dtype == dy_dtype), BF_EINVAL, "%s: dx may be dy only where their rows coincide", name);
     BF_REQUIRE(dx != dres || ld_dres == cols, BF_EINVAL, "%s: dx may be dres only where their rows coincide", name);
     const size_t ys = bf_dtype_size(dy_dtype), xs = bf_dtype_size(x_dtype), os = bf_dtype_size(dx_dtype);

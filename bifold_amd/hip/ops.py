@@ -1059,29 +1059,37 @@ def gemm_fp8(a8: torch.Tensor, a_scale: torch.Tensor, b8: torch.Tensor, b_scale:
 
 
 # ----------------------------------------------------------------------------- rows of any leading dimension
-def _here(*named) -> None:
-    """Every (tensor, name) lives on the current device: the launch goes to that device's stream."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t, name in named:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
-        if t.device.index != dev:
-            raise RuntimeError(f"{name} lives on {t.device}, the current device is cuda:{dev}")
+def _launch_stream(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The current stream of the device that all these tensors must live on, which must be the current one.  (Raw handles:
+    a torch.cuda.Stream object costs as much as the launch, and the smallest calls of this section are launch-bound.)"""
+    dev = first.get_device()
+    if dev < 0:
+        raise RuntimeError(f"tensors must live on the GPU (got {first.device}); there is no CPU path")
+    if dev != torch._C._cuda_getDevice():
+        raise RuntimeError(f"tensors live on {first.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"all tensors of a call live on one GPU: {first.device} and {t.device}")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of t's shape."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _row_layout(t: torch.Tensor, name: str):
     """(rows, cols, leading dimension) of a tensor whose last dimension is a row: contiguous, or 2-D with unit inner stride."""
-    if t.dim() < 1 or t.shape[-1] == 0:
-        raise RuntimeError(f"{name} needs a last dimension of at least one element, got {tuple(t.shape)}")
-    cols = t.shape[-1]
+    shape = t.shape
+    if not shape or shape[-1] == 0:
+        raise RuntimeError(f"{name} needs a last dimension of at least one element, got {tuple(shape)}")
+    cols = shape[-1]
     if t.is_contiguous():
         return t.numel() // cols, cols, cols
-    if t.dim() == 2 and (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or t.shape[0] == 1):
-        return t.shape[0], cols, t.stride(0) if t.shape[0] > 1 else cols
+    if len(shape) == 2 and (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or shape[0] == 1):
+        return shape[0], cols, t.stride(0) if shape[0] > 1 else cols
     raise RuntimeError(f"{name} must be contiguous, or 2-D with unit inner stride and rows that do not overlap, got "
-                       f"{tuple(t.shape)} {t.stride()}")
+                       f"{tuple(shape)} {t.stride()}")
 
 
 def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
@@ -1090,19 +1098,25 @@ def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     return t
 
 
+def _span(t: torch.Tensor):
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.numel() * t.element_size()
+    return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do the address ranges of two tensors meet?  (Strided views count from their first to their last element.)"""
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
     if a.numel() == 0 or b.numel() == 0:
         return False
-    (a0, a1), (b0, b1) = span(a), span(b)
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
 
 
-def _same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+def _apart_or_same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Is `a` memory of its own, or b itself (each element at the same address)?"""
+    return a is b or not _overlap(a, b) or (a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+                                            and a.dtype == b.dtype)
 
 
 # ----------------------------------------------------------------------------- 8-bit activation checkpoints
@@ -1111,10 +1125,9 @@ _GELUS = (L.ACT_QUICK_GELU, L.ACT_ERF_GELU, L.ACT_TANH_GELU)
 Checkpoint = Tuple[torch.Tensor, torch.Tensor]
 
 
-def _act8_empty(shape, device) -> Checkpoint:
-    groups = (shape[-1] + ACT8_GROUP - 1) // ACT8_GROUP
-    return (torch.empty(shape, dtype=torch.int8, device=device),
-            torch.empty(tuple(shape[:-1]) + (groups,), dtype=torch.uint8, device=device))
+def _act8_empty(x: torch.Tensor) -> Checkpoint:
+    shape = x.shape
+    return _like(x, torch.int8), x.new_empty((*shape[:-1], (shape[-1] + ACT8_GROUP - 1) // ACT8_GROUP), dtype=torch.uint8)
 
 
 def _act8_parts(kept: Checkpoint):
@@ -1131,10 +1144,9 @@ def act8_pack(x: torch.Tensor) -> Checkpoint:
     """The 8-bit checkpoint (q int8, code uint8) of x [..., cols], 33/32 bytes per element: groups of 32 columns share a
     power of two 2^e (code = e + 127), q = round(x 2^-e); see bf_act8_pack."""
     rows, cols, ld = _row_layout(x, "x")
-    _here((x, "x"))
-    q, code = _act8_empty(x.shape, x.device)
-    check(lib.bf_act8_pack(x.data_ptr(), ld, dtype_code(x), q.data_ptr(), code.data_ptr(), rows, cols, _stream()),
-          "bf_act8_pack")
+    stream = _launch_stream(x)
+    q, code = _act8_empty(x)
+    check(lib.bf_act8_pack(x.data_ptr(), ld, dtype_code(x), q.data_ptr(), code.data_ptr(), rows, cols, stream), "bf_act8_pack")
     return q, code
 
 
@@ -1142,13 +1154,12 @@ def act8_unpack(kept: Checkpoint, dtype: torch.dtype, out: Optional[torch.Tensor
     """The tensor a checkpoint stands for: q 2^e (exact in fp32 and bf16; NaN throughout a group that was not finite)."""
     q, code = _act8_parts(kept)
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        out = _like(q, dtype)
     elif out.shape != q.shape or out.dtype != dtype:
         raise RuntimeError(f"act8_unpack: out must be {dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
     rows, cols, ld = _row_layout(out, "out")
-    _here((q, "q"), (code, "code"), (out, "out"))
-    check(lib.bf_act8_unpack(q.data_ptr(), code.data_ptr(), out.data_ptr(), ld, dtype_code(out), rows, cols, _stream()),
-          "bf_act8_unpack")
+    check(lib.bf_act8_unpack(q.data_ptr(), code.data_ptr(), out.data_ptr(), ld, dtype_code(out), rows, cols,
+                             _launch_stream(q, code, out)), "bf_act8_unpack")
     return out
 
 
@@ -1156,11 +1167,11 @@ def act8_gelu_fwd(pre: torch.Tensor, act: int) -> Tuple[torch.Tensor, Checkpoint
     """(y, checkpoint of pre) with y = act(pre) in pre's dtype, in one pass; act: ACT_QUICK_GELU, ACT_ERF_GELU or
     ACT_TANH_GELU."""
     rows, cols, ld = _row_layout(pre, "pre")
-    _here((pre, "pre"))
-    y = torch.empty(pre.shape, dtype=pre.dtype, device=pre.device)
-    q, code = _act8_empty(pre.shape, pre.device)
+    stream = _launch_stream(pre)
+    y = _like(pre, pre.dtype)
+    q, code = _act8_empty(pre)
     check(lib.bf_act8_gelu_fwd(pre.data_ptr(), ld, y.data_ptr(), q.data_ptr(), code.data_ptr(), dtype_code(pre), act, rows, cols,
-                               _stream()), "bf_act8_gelu_fwd")
+                               stream), "bf_act8_gelu_fwd")
     return y, (q, code)
 
 
@@ -1171,13 +1182,13 @@ def act8_gelu_bwd(dy: torch.Tensor, kept: Checkpoint, act: int, out: Optional[to
         raise RuntimeError(f"act8_gelu_bwd: dy {tuple(dy.shape)} does not match the checkpoint {tuple(q.shape)}")
     rows, cols, ld = _row_layout(dy, "dy")
     if out is None:
-        out = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    elif out.shape != dy.shape or out.dtype != dy.dtype or (_overlap(out, dy) and not _same_rows(out, dy)):
+        out, ldo = _like(dy, dy.dtype), cols
+    elif out.shape != dy.shape or out.dtype != dy.dtype or not _apart_or_same(out, dy) or _overlap(out, q) or _overlap(out, code):
         raise RuntimeError("act8_gelu_bwd: out has dy's shape and dtype, and is dy or memory of its own")
-    _, _, ldo = _row_layout(out, "out")
-    _here((dy, "dy"), (q, "q"), (code, "code"), (out, "out"))
+    else:
+        _, _, ldo = _row_layout(out, "out")
     check(lib.bf_act8_gelu_bwd(dy.data_ptr(), ld, q.data_ptr(), code.data_ptr(), out.data_ptr(), ldo, dtype_code(dy), act, rows,
-                               cols, _stream()), "bf_act8_gelu_bwd")
+                               cols, _launch_stream(dy, q, code, out)), "bf_act8_gelu_bwd")
     return out
 
 
@@ -1199,15 +1210,16 @@ def _rms_args(x, gamma, delta, x_out, write_x):
             x_out = None
         else:
             if x_out is None:
-                x_out = x
-            elif x_out.shape != x.shape or x_out.dtype != x.dtype:
-                raise RuntimeError("rmsnorm: x_out has x's shape and dtype")
-            for t, name in ((x, "x"), (delta, "delta")):
-                if _overlap(x_out, t) and not _same_rows(x_out, t):
-                    raise RuntimeError(f"rmsnorm: x_out is {name} or memory of its own")
-            _, _, ldo = _row_layout(x_out, "x_out")
-    _here((x, "x"), (gamma, "gamma"), (delta, "delta"), (x_out, "x_out"))
-    return rows, cols, ldx, ldd, d_dtype, ldo, x_out
+                x_out, ldo = x, ldx
+            else:
+                if x_out.shape != x.shape or x_out.dtype != x.dtype:
+                    raise RuntimeError("rmsnorm: x_out has x's shape and dtype")
+                if not _apart_or_same(x_out, x):
+                    raise RuntimeError("rmsnorm: x_out is x or memory of its own")
+                _, _, ldo = _row_layout(x_out, "x_out")
+            if not _apart_or_same(x_out, delta):
+                raise RuntimeError("rmsnorm: x_out is delta or memory of its own")
+    return rows, cols, ldx, ldd, d_dtype, ldo, x_out, _launch_stream(x, gamma, delta, x_out)
 
 
 def rmsnorm_fwd(x: torch.Tensor, gamma: torch.Tensor, out_dtype: torch.dtype, delta: Optional[torch.Tensor] = None,
@@ -1216,12 +1228,12 @@ def rmsnorm_fwd(x: torch.Tensor, gamma: torch.Tensor, out_dtype: torch.dtype, de
     """t = x + delta; y = t / sqrt(mean(t^2) + eps) * gamma over the last dimension.  x_out = t rounded to x's dtype: given,
     or x itself (in place) when None, or not written (write_x=False; also without a delta).  `checkpoint`: also the 8-bit
     checkpoint of t.  Returns (y, rstd or None, checkpoint or None)."""
-    rows, cols, ldx, ldd, d_dtype, ldo, x_out = _rms_args(x, gamma, delta, x_out, write_x)
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if save_stats else None
-    q, code = _act8_empty(x.shape, x.device) if checkpoint else (None, None)
+    rows, cols, ldx, ldd, d_dtype, ldo, x_out, stream = _rms_args(x, gamma, delta, x_out, write_x)
+    y = _like(x, out_dtype)
+    rstd = gamma.new_empty(rows) if save_stats else None
+    q, code = _act8_empty(x) if checkpoint else (None, None)
     check(lib.bf_rmsnorm_fwd(x.data_ptr(), ldx, dtype_code(x), _ptr(delta), ldd, d_dtype, gamma.data_ptr(), _ptr(x_out), ldo,
-                             y.data_ptr(), dtype_code(y), _ptr(rstd), _ptr(q), _ptr(code), rows, cols, eps, _stream()),
+                             y.data_ptr(), dtype_code(y), _ptr(rstd), _ptr(q), _ptr(code), rows, cols, eps, stream),
           "bf_rmsnorm_fwd")
     return y, rstd, (q, code) if checkpoint else None
 
@@ -1231,14 +1243,14 @@ def rmsnorm_fwd_fp8(x: torch.Tensor, gamma: torch.Tensor, delta: Optional[torch.
                     checkpoint: bool = False):
     """rmsnorm_fwd with e4m3 output for ops.gemm_fp8: returns (y uint8, row scales fp32 [rows], rstd or None, checkpoint or
     None); y ~= bytes * scale, scale = max |y| / 448 of the row."""
-    rows, cols, ldx, ldd, d_dtype, ldo, x_out = _rms_args(x, gamma, delta, x_out, write_x)
-    y = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if save_stats else None
-    q, code = _act8_empty(x.shape, x.device) if checkpoint else (None, None)
+    rows, cols, ldx, ldd, d_dtype, ldo, x_out, stream = _rms_args(x, gamma, delta, x_out, write_x)
+    y = _like(x, torch.uint8)
+    scale = gamma.new_empty(rows)
+    rstd = gamma.new_empty(rows) if save_stats else None
+    q, code = _act8_empty(x) if checkpoint else (None, None)
     check(lib.bf_rmsnorm_fwd_fp8(x.data_ptr(), ldx, dtype_code(x), _ptr(delta), ldd, d_dtype, gamma.data_ptr(), _ptr(x_out),
                                  ldo, y.data_ptr(), scale.data_ptr(), _ptr(rstd), _ptr(q), _ptr(code), rows, cols, eps,
-                                 _stream()), "bf_rmsnorm_fwd_fp8")
+                                 stream), "bf_rmsnorm_fwd_fp8")
     return y, scale, rstd, (q, code) if checkpoint else None
 
 
@@ -1263,22 +1275,21 @@ def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dg
     if dres is not None:
         _, _, ldr = _row_layout(dres, "dres")
     if out is None:
-        out = torch.empty(dy.shape, dtype=dt, device=dy.device)
+        out = _like(dy, dt)
     else:
         if out.shape != dy.shape or out.dtype != dt or not out.is_contiguous():
             raise RuntimeError(f"rmsnorm_bwd: out must be a contiguous {dt} tensor of dy's shape")
         for t, name in ((dy, "dy"), (dres, "dres")):
-            if t is not None and _overlap(out, t) and not (_same_rows(out, t) and (name == "dres" or cols <= 8192)):
-                raise RuntimeError(f"rmsnorm_bwd: out is {name} (dy: up to 8192 columns) or memory of its own")
+            if t is not None and not _apart_or_same(out, t):
+                raise RuntimeError(f"rmsnorm_bwd: out is {name} or memory of its own")
         for t in (x, q, code, gamma, rstd, dgamma_out):
             if t is not None and _overlap(out, t):
                 raise RuntimeError("rmsnorm_bwd: out must not overlap x, the checkpoint, gamma, rstd or dgamma_out")
-    _here((dy, "dy"), (x, "x"), (q, "q"), (code, "code"), (gamma, "gamma"), (rstd, "rstd"), (dres, "dres"), (out, "out"),
-          (dgamma_out, "dgamma_out"))
-    parts = torch.empty(lib.bf_rmsnorm_bwd_parts(rows, cols), cols, dtype=torch.float32, device=dy.device)
+    stream = _launch_stream(dy, x, q, code, gamma, rstd, dres, out, dgamma_out)
+    parts = gamma.new_empty(lib.bf_rmsnorm_bwd_parts(rows, cols) * cols)
     check(lib.bf_rmsnorm_bwd(dy.data_ptr(), ldy, dtype_code(dy), _ptr(x), ldx, x_dtype, _ptr(q), _ptr(code), gamma.data_ptr(),
                              rstd.data_ptr(), _ptr(dres), ldr, out.data_ptr(), dtype_code(out), dgamma_out.data_ptr(),
-                             parts.data_ptr(), rows, cols, _stream()), "bf_rmsnorm_bwd")
+                             parts.data_ptr(), rows, cols, stream), "bf_rmsnorm_bwd")
     return out
 
 
@@ -1301,11 +1312,11 @@ def embed_scaled_fwd(tokens: torch.Tensor, table: torch.Tensor, scale: float, er
     _flag(err_flag)
     if table.dim() != 2 or not table.is_contiguous() or 0 in table.shape:
         raise RuntimeError(f"embed_scaled_fwd: table must be a contiguous [vocab, cols] tensor, got {tuple(table.shape)}")
-    _here((tokens, "tokens"), (table, "table"), (err_flag, "err_flag"))
+    stream = _launch_stream(tokens, table, err_flag)
     vocab, cols = table.shape
-    out = torch.empty(n, cols, dtype=out_dtype or table.dtype, device=table.device)
+    out = table.new_empty((n, cols), dtype=out_dtype or table.dtype)
     check(lib.bf_embed_scaled_fwd(tokens.data_ptr(), table.data_ptr(), dtype_code(table), out.data_ptr(), dtype_code(out),
-                                  scale, n, cols, vocab, _ptr(err_flag), _stream()), "bf_embed_scaled_fwd")
+                                  scale, n, cols, vocab, _ptr(err_flag), stream), "bf_embed_scaled_fwd")
     return out
 
 
@@ -1325,13 +1336,13 @@ def embed_scaled_bwd(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: 
     if out is None:
         if accumulate:
             raise RuntimeError("accumulate needs an `out` to add into")
-        out = torch.empty(vocab, cols, dtype=torch.float32, device=dy.device)
+        out = dy.new_empty((vocab, cols), dtype=torch.float32)
     elif out.dtype != torch.float32 or tuple(out.shape) != (vocab, cols) or not out.is_contiguous() or _overlap(out, dy):
         raise RuntimeError(f"embed_scaled_bwd: out must be a contiguous float32 {(vocab, cols)} tensor apart from dy")
-    _here((dy, "dy"), (tokens, "tokens"), (out, "out"), (err_flag, "err_flag"))
+    stream = _launch_stream(dy, tokens, out, err_flag)
     need = lib.bf_embed_scaled_bwd_workspace_bytes(n, cols, vocab)
-    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    ws = dy.new_empty(need, dtype=torch.uint8) if need else None
     check(lib.bf_embed_scaled_bwd(dy.data_ptr(), ld, dtype_code(dy), tokens.data_ptr(), out.data_ptr(), scale, int(accumulate),
                                   -1 if padding_idx is None else padding_idx, n, cols, vocab, _ptr(err_flag), _ptr(ws), need,
-                                  _stream()), "bf_embed_scaled_bwd")
+                                  stream), "bf_embed_scaled_bwd")
     return out

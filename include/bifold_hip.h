@@ -676,7 +676,7 @@ int bf_act8_gelu_bwd(const void* dy, int64_t ld_dy, const void* q, const void* c
  *   infinity): bf_gemm_fp8's operand, as bf_layernorm_fwd_fp8 writes it.
  * bwd:  h = t r;  b = dy gamma;  dx = dres + r (b - h mean(b h));  dgamma [cols] = sum over rows of dy h (overwritten; summed
  *   in a fixed order).  The stream t is x, or a checkpoint q / code with x = NULL; dres (of dx's type) may be NULL; dx may be
- *   dres, and up to 8 192 columns dy, where their rows coincide.  parts_ws: bf_rmsnorm_bwd_parts(rows, cols) * cols floats. */
+ *   dres or dy where their rows coincide.  parts_ws: bf_rmsnorm_bwd_parts(rows, cols) * cols floats. */
 int bf_rmsnorm_fwd(const void* x, int64_t ldx, int x_dtype, const void* delta, int64_t ld_delta, int delta_dtype, const float* gamma,
                    void* x_out, int64_t ld_out, void* y, int y_dtype, float* rstd, void* q, void* code, int rows, int cols,
                    float eps, bf_stream_t stream);

@@ -73,7 +73,6 @@ def test_rmsnorm_refusals(L):
     refused(L, bwd(dx=PTR, ldy=72), -1, "rows coincide")
     refused(L, bwd(dx=PTR, dxd=L.F32), -1, "rows coincide")
     refused(L, bwd(dres=2 * PTR, ldr=72), -1, "rows coincide")
-    refused(L, bwd(dx=PTR, cols=8200, ldy=8200, ldx=8200), -1, "8192")
     refused(L, bwd(rstd=PTR + 1), -2, "aligned")
     assert [lib.bf_rmsnorm_bwd_parts(r, c) for r, c in ((0, 64), (1, 64), (5, 64), (10 ** 6, 64), (7, 4096), (9000, 4096),
                                                          (9000, 9000))] == [0, 1, 2, 1024, 7, 512, 64]
@@ -105,7 +104,7 @@ def test_embedding_refusals(L):
     assert bwd(n=0, dy=None, ids=None) == 0
     size = lib.bf_embed_scaled_bwd_workspace_bytes
     assert size(512, 64, 100) == 0 and size(513, 64, 100) > 16 * 513
-    assert size(1 << 20, 1024, 1 << 20) < 1 << 28
+    assert size(1 << 20, 1024, 1 << 20) < 1 << 29
 
 
 def test_wrappers_refuse_before_the_library(L):

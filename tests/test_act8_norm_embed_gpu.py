@@ -323,7 +323,8 @@ def rms_bwd_ref(dy, t, r, gamma, dres):
 @pytest.mark.parametrize("dyd,xd,rd", [(torch.float32, torch.float32, torch.float32), (torch.float16, torch.float32, torch.float16),
                                        (torch.bfloat16, "kept", torch.bfloat16), (torch.float16, "kept", torch.float32),
                                        (torch.float32, "kept", None), (torch.bfloat16, torch.bfloat16, None),
-                                       (torch.float16, torch.float16, torch.float16)])
+                                       (torch.float16, torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16, torch.float32),
+                                       (torch.float32, torch.bfloat16, torch.bfloat16), (torch.float16, torch.bfloat16, None)])
 @pytest.mark.parametrize("layout", ["plain", "off"])
 def test_rmsnorm_bwd(ops, gpu, rows, cols, dyd, xd, rd, layout):
     eps = 1e-6
@@ -354,7 +355,7 @@ def test_rmsnorm_bwd(ops, gpu, rows, cols, dyd, xd, rd, layout):
         into = dres.clone()
         assert ops.rmsnorm_bwd(dy, kept if xd == "kept" else src, gamma.to(gpu), rstd, dg, dres=into, out=into) is into
         assert torch.equal(into, dx)
-    if layout == "plain" and dyd == od and cols <= 8192:
+    if layout == "plain" and dyd == od:
         into = dy.clone()
         assert ops.rmsnorm_bwd(into, kept if xd == "kept" else src, gamma.to(gpu), rstd, dg, dres=dres, out=into) is into
         assert torch.equal(into, dx)
