@@ -4,8 +4,10 @@
 //   bf_act8_gelu_fwd   pre -> y = act(pre), and the checkpoint of pre, in one pass
 //   bf_act8_gelu_bwd   dy, checkpoint -> dpre = dy act'(q 2^e)
 // All four stream: every byte is touched once and nothing is reused, so HBM bounds them and the layout is chosen for it.  A
-// lane holds 8 consecutive elements (one 16-byte access of a 16-bit tensor, two of an fp32 one, 8 bytes of q); a group of 32
-// is a quad of lanes, its maximum two cross-lane moves without LDS.
+// lane holds V = 8 consecutive elements (one 16-byte access of a 16-bit tensor, 8 bytes of q) or 4 of an fp32 tensor; a group
+// of 32 is a quad of lanes (or two), its maximum two (three) cross-lane moves without LDS.  One vector a lane and many
+// workgroups: with four vectors a lane in flight the same kernels took 129 and 159 us where they take 119 and 137 (forward
+// and backward of 36 928 x 4 096 fp16: 6.4 and 5.6 TB/s; a copy of 2 GiB reaches 4.9, one of 256 MiB 5.5).
 #include "act8.h"
 
 namespace {
@@ -46,7 +48,7 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float act_slope(float 
 
 // One kernel body for the four: MODE picks what is read and written.  DENSE: cols is a multiple of 32, all rows follow each
 // other and are 16-byte aligned, so vector v lies at element 8 v.  Otherwise a row owns a whole number of quads of lanes
-// (the last ones partly or wholly empty), `vpr` per row, and accesses may be unaligned: one division per 8 elements.
+// (the last ones partly or wholly empty), `vpr` vectors of 8 per row, and accesses may be unaligned: one division per vector.
 struct A8Args {
     const void* x; int64_t ldx;             // A8_PACK / A8_FWD: the activation;  A8_BWD: dy
     void* y; int64_t ldy;                   // A8_FWD: act(pre);  A8_BWD: dpre;  A8_UNPACK: the tensor
@@ -54,73 +56,69 @@ struct A8Args {
     unsigned nvec; unsigned vpr; int cols; int gpr;
 };
 
-template <typename T, int MODE, int ACT, bool DENSE, int U>
+template <typename T, int MODE, int ACT, bool DENSE, int V>
 __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
     constexpr bool EXACT = sizeof(T) == 4;
-    const unsigned v0 = blockIdx.x * (256u * U) + threadIdx.x;
-    const T* x = (const T*)a.x;
-    T* y = (T*)a.y;
-    float f[U][8];
-    unsigned w[U][2], code[U];
-    size_t off_x[U], off_y[U], off_q[U], off_c[U];
-    int n[U];
-    bool first[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned v = v0 + u * 256u;
-        n[u] = v < a.nvec ? 8 : 0;
-        if constexpr (DENSE) {
-            off_x[u] = off_y[u] = off_q[u] = (size_t)v * 8;
-            off_c[u] = v >> 2;
-            first[u] = (v & 3) == 0 && n[u] > 0;
-        } else {
-            const unsigned row = v / a.vpr, c = (v - row * a.vpr) * 8;
-            if (n[u]) n[u] = min(8, a.cols - (int)c);          // <= 0 in the lanes that fill up the row's last group
-            off_x[u] = (size_t)row * a.ldx + c;
-            off_y[u] = (size_t)row * a.ldy + c;
-            off_q[u] = (size_t)row * a.cols + c;
-            off_c[u] = (size_t)row * a.gpr + (c >> 5);
-            first[u] = (c & 31) == 0 && n[u] > 0;
-        }
-        if constexpr (MODE == A8_UNPACK || MODE == A8_BWD) {
-            bytes_load_n<8, DENSE>(a.q + off_q[u], n[u], w[u]);
-            code[u] = n[u] > 0 ? a.code[off_c[u]] : 1u;
-        }
-        if constexpr (MODE != A8_UNPACK) vec_load_n<T, 8, DENSE>(x + off_x[u], n[u], f[u]);
+    constexpr unsigned PER = ACT8_GROUP / V;                   // lanes per group
+    const unsigned v = blockIdx.x * 256u + threadIdx.x;
+    int n = v < a.nvec ? V : 0;
+    size_t off_x, off_y, off_q, off_c;
+    bool first;
+    if constexpr (DENSE) {
+        off_x = off_y = off_q = (size_t)v * V;
+        off_c = v / PER;
+        first = v % PER == 0 && n > 0;
+    } else {
+        const unsigned row = v / a.vpr, c = (v - row * a.vpr) * V;
+        if (n) n = min(V, a.cols - (int)c);                    // <= 0 in the lanes that fill up the row's last group
+        off_x = (size_t)row * a.ldx + c;
+        off_y = (size_t)row * a.ldy + c;
+        off_q = (size_t)row * a.cols + c;
+        off_c = (size_t)row * a.gpr + c / ACT8_GROUP;
+        first = c % ACT8_GROUP == 0 && n > 0;
     }
+    const T* x = (const T*)a.x + off_x;
+    T* y = (T*)a.y + off_y;
+    float f[V];
+    unsigned w[V / 4], code;
+    if constexpr (MODE == A8_PACK || MODE == A8_FWD) {
+        vec_load_n<T, V, DENSE>(x, n, f);
+        code = act8_code(group_max<V>(magnitude_bits<V>(f)));
+        act8_quant<V>(f, code, w);
+        bytes_store_n<V, DENSE>(a.q + off_q, n, w);
+        if (first) a.code[off_c] = (uint8_t)code;
+        if constexpr (MODE == A8_FWD) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if constexpr (MODE == A8_PACK || MODE == A8_FWD) {
-            code[u] = act8_code(group_max<8>(magnitude_bits<8>(f[u])));
-            act8_quant<8>(f[u], code[u], w[u]);
-            bytes_store_n<8, DENSE>(a.q + off_q[u], n[u], w[u]);
-            if (first[u]) a.code[off_c[u]] = (uint8_t)code[u];
-            if constexpr (MODE == A8_FWD) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[u][j] = act_value<ACT, EXACT>(f[u][j]);
-                vec_store_n<T, 8, DENSE>(y + off_y[u], n[u], f[u]);
-            }
-        } else {
-            float k[8];
-            act8_dequant<8>(w[u], code[u], k);
-            if constexpr (MODE == A8_BWD) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) k[j] = f[u][j] * act_slope<ACT, EXACT>(k[j]);
-            }
-            vec_store_n<T, 8, DENSE>(y + off_y[u], n[u], k);
+            for (int j = 0; j < V; ++j) f[j] = act_value<ACT, EXACT>(f[j]);
+            vec_store_n<T, V, DENSE>(y, n, f);
         }
+    } else {
+        Chunk<T, V, DENSE> dy;
+        bytes_load_n<V, DENSE>(a.q + off_q, n, w);
+        code = n > 0 ? a.code[off_c] : 1u;
+        if constexpr (MODE == A8_BWD) dy.load(x, 0, n);
+        act8_dequant<V>(w, code, f);
+        if constexpr (MODE == A8_BWD) {
+            float d[V];
+            dy.take(d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = d[j] * act_slope<ACT, EXACT>(f[j]);
+        }
+        vec_store_n<T, V, DENSE>(y, n, f);
     }
 }
 
 template <typename T, int MODE, int ACT>
 void act8_launch(const A8Args& a, bool dense, hipStream_t s) {
-    // DENSE: four vectors per thread keep four (fp32: eight) 16-byte loads in flight per lane; two where addresses cost registers
     if (dense) {
-        const unsigned blocks = (unsigned)(((size_t)a.nvec + 1023) / 1024);
-        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, true, 4>), dim3(blocks), dim3(256), 0, s, a);
+        // fp32 writers of q take 4 elements a lane (whole lines per load instruction): 73 728 x 768 packed in 56.4 us, with 8
+        // in 61.5; the read-back takes 8 (44.7 us, with 4 in 47.8)
+        constexpr int V = sizeof(T) == 4 && MODE != A8_UNPACK ? 4 : 8;
+        A8Args b = a;
+        b.nvec = a.nvec * (8 / V);
+        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, true, V>), dim3((unsigned)(((size_t)b.nvec + 255) / 256)), dim3(256), 0, s, b);
     } else {
-        const unsigned blocks = (unsigned)(((size_t)a.nvec + 511) / 512);
-        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, false, 2>), dim3(blocks), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, false, 8>), dim3((unsigned)(((size_t)a.nvec + 255) / 256)), dim3(256), 0, s, a);
     }
 }
 
@@ -151,7 +149,7 @@ int act8_run(const char* name, const void* x, int64_t ldx, void* y, int64_t ldy,
     a.cols = cols; a.gpr = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
     a.vpr = (unsigned)a.gpr * 4;
     const unsigned long long nvec = (unsigned long long)rows * a.vpr;
-    BF_REQUIRE(nvec <= 0xFFFFF000ull, BF_EINVAL, "%s: rows=%lld x cols=%d is over 2^35 elements", name, (long long)rows, cols);
+    BF_REQUIRE(nvec <= 0x7FFFF000ull, BF_EINVAL, "%s: rows=%lld x cols=%d is over 2^34 elements", name, (long long)rows, cols);
     a.nvec = (unsigned)nvec;
     const bool dense = cols % ACT8_GROUP == 0 && (!HAS_X || (ldx == cols && bf_aligned16(x))) &&
                        (!HAS_Y || (ldy == cols && bf_aligned16(y))) && ((uintptr_t)q & 7u) == 0;

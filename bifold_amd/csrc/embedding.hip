@@ -15,34 +15,24 @@ template <typename TT, bool AL>
 __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __restrict__ ids, const TT* __restrict__ table,
                                                            void* __restrict__ out, int out_dtype, float scale, unsigned nvec,
                                                            unsigned vpr, int cols, int vocab, int* __restrict__ err_flag) {
-    constexpr int V = sizeof(TT) == 4 ? 4 : 8, U = 4;
-    float f[U][V];
-    size_t off[U];
-    int n[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned v = blockIdx.x * (256u * U) + u * 256u + threadIdx.x;
-        const unsigned row = v / vpr, c = (v - row * vpr) * V;
-        n[u] = v < nvec ? cols - (int)c : 0;
-        off[u] = (size_t)row * cols + c;
-        int id = 0;
-        if (n[u] > 0) {
-            id = ids[row];
-            if (id < 0 || id >= vocab) {
-                if (c == 0 && err_flag) atomicExch(err_flag, 1);
-                id = 0;
-            }
-        }
-        vec_load_n<TT, V, AL>(table + (size_t)id * cols + c, n[u], f[u]);
+    constexpr int V = sizeof(TT) == 4 ? 4 : 8;
+    const unsigned v = blockIdx.x * 256u + threadIdx.x;
+    if (v >= nvec) return;
+    const unsigned row = v / vpr, c = (v - row * vpr) * V;
+    const int n = cols - (int)c;
+    int id = ids[row];
+    if (id < 0 || id >= vocab) {
+        if (c == 0 && err_flag) atomicExch(err_flag, 1);
+        id = 0;
     }
+    float f[V];
+    vec_load_n<TT, V, AL>(table + (size_t)id * cols + c, n, f);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[u][j] *= scale;
-        if (out_dtype == BF_F32) vec_store_n<float, V, AL>((float*)out + off[u], n[u], f[u]);
-        else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)out + off[u], n[u], f[u]);
-        else vec_store_n<f16_t, V, AL>((f16_t*)out + off[u], n[u], f[u]);
-    }
+    for (int j = 0; j < V; ++j) f[j] *= scale;
+    const size_t off = (size_t)row * cols + c;
+    if (out_dtype == BF_F32) vec_store_n<float, V, AL>((float*)out + off, n, f);
+    else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)out + off, n, f);
+    else vec_store_n<f16_t, V, AL>((f16_t*)out + off, n, f);
 }
 
 // ------------------------------------------------------------------ zeros of the dense gradient
@@ -475,7 +465,7 @@ extern "C" int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int
     const unsigned long long nvec = (unsigned long long)n * vpr;
     BF_REQUIRE(nvec <= 0xFFFFF000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
     const bool al = cols % V == 0 && bf_aligned16(table) && bf_aligned16(out);
-    const dim3 grid((unsigned)((nvec + 1023) / 1024)), block(256);
+    const dim3 grid((unsigned)((nvec + 255) / 256)), block(256);
     hipStream_t s = (hipStream_t)stream;
 #define EMBED_FWD(T)                                                                                                             \
     do {                                                                                                                         \

@@ -27,7 +27,7 @@ def test_act8_refusals(L):
     refused(L, lib.bf_act8_pack(None, 64, L.F32, PTR, PTR, 4, 64, None), -1, "null")
     refused(L, lib.bf_act8_pack(PTR, 64, L.F32, PTR, None, 4, 64, None), -1, "null")
     refused(L, lib.bf_act8_pack(PTR + 2, 64, L.F32, PTR, PTR, 4, 64, None), -2, "aligned")
-    refused(L, lib.bf_act8_pack(PTR, 32, L.F16, PTR, PTR, 1 << 30, 32, None), -1, "2^35")
+    refused(L, lib.bf_act8_pack(PTR, 32, L.F16, PTR, PTR, 1 << 30, 32, None), -1, "2^34")
     refused(L, lib.bf_act8_unpack(PTR, PTR, PTR, 63, L.F16, 4, 64, None), -1, "leading dimension")
     refused(L, lib.bf_act8_unpack(PTR, PTR, PTR + 1, 64, L.F16, 4, 64, None), -2, "aligned")
     for act in (L.ACT_NONE, 3, 5, 99):
