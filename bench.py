@@ -298,6 +298,8 @@ def main():
     ap.add_argument("--lora-recompute", default="none", choices=["none", "mlp", "full"],
                     help="siglip_seq --lora: what the towers' backward re-makes instead of keeping (none 198 samples/s at "
                          "181 GiB, mlp 190 at 147 GiB, full 179 at 109 GiB; B = 128)")
+    ap.add_argument("--lora-checkpoint", default="native", choices=["native", "int8"],
+                    help="siglip_seq --lora: keep the towers' activations in their own types or in 8 bits")
     ap.add_argument("--mask-head", action="store_true",
                     help="diagnostic (configs a / vitl14): PickPlaceConvDecoder(compute_mask=True) under the reference's "
                          "conf/loss/composed_dice_focal.yaml (bce_gaussmap x 40 with mask_pick_heatmap, focal x 20, dice x 1) "
@@ -345,7 +347,7 @@ def main():
                        lora_alpha=32, lora_dropout=(args.lora_dropout if args.lora else 0.0), target_modules=["q_proj", "v_proj"], threshold=0.5,
                        text_encoder=None, pick_place_model="pick_place_convdecoder", fusion_model="concat_transformer",
                        depth=8, heads=16, mlp_ratio=4, dropout=0.0, dtype=dtype, context_length=4,
-                       lora_recompute=args.lora_recompute)
+                       lora_recompute=args.lora_recompute, lora_checkpoint=args.lora_checkpoint)
         if args.mask_head:
             if seq or fp8:
                 raise SystemExit("--mask-head goes with --config a / vitl14")

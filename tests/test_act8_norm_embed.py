@@ -160,3 +160,14 @@ def test_wrappers_refuse_before_the_library(L):
         ops.embed_scaled_bwd(x, ids, 10, 1.0, accumulate=True)
     with pytest.raises(RuntimeError, match="apart from dy"):
         ops.embed_scaled_bwd(x, ids, 10, 1.0, out=torch.zeros(9, 64))
+
+
+def test_lora_checkpoint_values():
+    from bifold.models.siglip_encoder import SiglipTowers
+    tower = dict(hidden_size=64, intermediate_size=128, num_hidden_layers=1, num_attention_heads=2)
+    vision, text = dict(tower, image_size=32, patch_size=16), dict(tower, vocab_size=100, max_position_embeddings=64)
+    lora = dict(r=8, alpha=32, targets=["q_proj", "v_proj"])
+    assert SiglipTowers(vision, text, lora=lora).lora["checkpoint"] == "native"
+    assert SiglipTowers(vision, text, lora=dict(lora, checkpoint="int8")).lora["checkpoint"] == "int8"
+    with pytest.raises(ValueError, match="native or int8"):
+        SiglipTowers(vision, text, lora=dict(lora, checkpoint="int4"))

@@ -614,3 +614,59 @@ def test_block_from_tokens_to_table_gradient(ops, L, gpu):
     wt = torch.zeros(vocab, width, dtype=torch.float64).index_add_(0, ids, dxr) * scale
     size = torch.zeros(vocab, width, dtype=torch.float64).index_add_(0, ids, dxr.abs()) * scale
     close(grad, wt, U * (torch.bincount(ids, minlength=vocab).double()[:, None] + 2) * size, "table gradient")
+
+
+# ------------------------------------------------------------------ the LoRA towers' backward from 8-bit checkpoints
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("p_drop", [0.0, 0.25])
+@pytest.mark.parametrize("policy", ["none", "mlp", "full"])
+def test_lora_backward_from_checkpoints(ops, gpu, dtype, p_drop, policy):
+    """`lora_checkpoint: int8` changes nothing in the forward, and its backward is the one of `native` with every kept
+    activation replaced by what its checkpoint reads back as: the adapters' gradients are the same bits."""
+    from bifold.losses import Losses
+    from bifold.models import siglip_encoder
+    from test_model_gpu import build_tiny_siglip
+    T, B = 2, 2
+    loss_fn = Losses.get_by_name(cfg=dict(name="bce_gaussmap", is_bimanual=True, mask_pick_heatmap=False))
+    g = torch.Generator().manual_seed(77)
+    sample = {"rgb": torch.randn(B, 3, 32, 32, generator=g), "rgb_context": torch.randn(B, T, 3, 32, 32, generator=g),
+              "instruction": torch.randint(0, 100, (B, 64), generator=g),
+              "context_attention_mask": torch.tensor([[1, 0], [1, 1]])}
+    for hn in ("left_pick", "left_place", "right_pick", "right_place"):
+        sample[f"{hn}_heatmap"] = torch.rand(B, 32, 32, generator=g)
+    sample = {k: v.to(gpu) for k, v in sample.items()}
+    seen = {}
+    for how in ("native", "replaced", "int8"):
+        torch.manual_seed(5)
+        model = build_tiny_siglip("siglip_sequential", True, dtype, gpu, T, lora=True, r=8, lora_dropout=p_drop,
+                                  lora_recompute=policy, lora_checkpoint="int8" if how == "int8" else "native")
+        with torch.no_grad():
+            gb = torch.Generator().manual_seed(6)
+            for n, p in model.named_parameters():
+                if ".lora_B." in n:
+                    p.copy_(torch.randn(p.shape, generator=gb) * 0.05)
+        model = model.to(gpu).train()
+        torch.manual_seed(9)
+        out = model(sample)
+        loss, _ = loss_fn(out, sample)
+        kept = 0
+        for tower in model.siglip_model._saved.values():
+            for S in tower["layers"]:
+                for k in siglip_encoder._KEPT8:
+                    kept += S[k] is not None
+                    if S[k] is None:
+                        continue
+                    assert isinstance(S[k], tuple) == (how == "int8")
+                    if how == "replaced":
+                        S[k] = ops.act8_unpack(ops.act8_pack(S[k]), S[k].dtype)
+        assert kept == 2 * 2 * {"none": 4, "mlp": 2, "full": 1}[policy]
+        model.zero_grad()
+        loss.backward()
+        torch.cuda.synchronize()
+        seen[how] = (loss.detach().clone(), {n: p.grad.detach().clone() for n, p in model.named_parameters()
+                                             if p.requires_grad and ".lora_" in n})
+    assert torch.equal(seen["int8"][0], seen["native"][0]) and len(seen["int8"][1]) == 16
+    for n, gr in seen["replaced"][1].items():
+        assert torch.equal(seen["int8"][1][n], gr), n
+        assert torch.isfinite(gr).all() and gr.abs().max() > 0
+    assert any(not torch.equal(seen["int8"][1][n], gr) for n, gr in seen["native"][1].items())
