@@ -133,7 +133,7 @@ template <int MODE>
 int act8_run(const char* name, const void* x, int64_t ldx, void* y, int64_t ldy, void* q, void* code, int dtype, int act,
              int64_t rows, int cols, bf_stream_t stream) {
     BF_REQUIRE(dtype == BF_F32 || bf_is_half(dtype), BF_EINVAL, "%s: bad dtype %d", name, dtype);
-    BF_REQUIRE(rows >= 0 && cols > 0, BF_EINVAL, "%s: bad shape (rows=%lld cols=%d)", name, (long long)rows, cols);
+    BF_REQUIRE(rows >= 0 && cols > 0 && cols <= (1 << 30), BF_EINVAL, "%s: bad shape (rows=%lld cols=%d)", name, (long long)rows, cols);
     constexpr bool HAS_X = MODE != A8_UNPACK, HAS_Y = MODE != A8_PACK;
     BF_REQUIRE((!HAS_X || ldx >= cols) && (!HAS_Y || ldy >= cols), BF_EINVAL, "%s: a leading dimension is under cols=%d", name, cols);
     if (MODE == A8_FWD || MODE == A8_BWD)

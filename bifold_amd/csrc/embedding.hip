@@ -11,36 +11,44 @@
 namespace {
 
 // ------------------------------------------------------------------ lookup
-template <typename TT, bool AL>
+template <typename TT, bool AL, int U>
 __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __restrict__ ids, const TT* __restrict__ table,
                                                            void* __restrict__ out, int out_dtype, float scale, unsigned nvec,
                                                            unsigned vpr, int cols, int vocab, int* __restrict__ err_flag) {
     constexpr int V = sizeof(TT) == 4 ? 4 : 8;
-    const unsigned v = blockIdx.x * 256u + threadIdx.x;
-    if (v >= nvec) return;
-    const unsigned row = v / vpr, c = (v - row * vpr) * V;
-    const int n = cols - (int)c;
-    int id = ids[row];
-    if (id < 0 || id >= vocab) {
-        if (c == 0 && err_flag) atomicExch(err_flag, 1);
-        id = 0;
-    }
-    float f[V];
-    vec_load_n<TT, V, AL>(table + (size_t)id * cols + c, n, f);
+    // two dependent loads: all ids first, then all rows, no branch between (which would wait for each)
+    unsigned row[U], c[U];
+    int id[U];
+    Chunk<TT, V, AL> x[U];
+    const unsigned v0 = blockIdx.x * (256u * U) + threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] *= scale;
-    const size_t off = (size_t)row * cols + c;
-    if (out_dtype == BF_F32) vec_store_n<float, V, AL>((float*)out + off, n, f);
-    else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)out + off, n, f);
-    else vec_store_n<f16_t, V, AL>((f16_t*)out + off, n, f);
-}
-
-// ------------------------------------------------------------------ zeros of the dense gradient
-__global__ __launch_bounds__(512) void embed_zero_kernel(float* __restrict__ p, size_t n) {
-    const size_t at = (size_t)blockIdx.x * 512 + threadIdx.x, step = (size_t)gridDim.x * 512;
-    const size_t n4 = ((uintptr_t)p & 15u) == 0 ? n >> 2 : 0;
-    for (size_t i = at; i < n4; i += step) ((float4*)p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (size_t i = n4 * 4 + at; i < n; i += step) p[i] = 0.f;
+    for (int u = 0; u < U; ++u) {
+        const unsigned v = min(v0 + u * 256u, nvec - 1);
+        row[u] = v / vpr;
+        c[u] = (v - row[u] * vpr) * V;
+        id[u] = ids[row[u]];
+    }
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const bool out_of = id[u] < 0 || id[u] >= vocab;
+        bad |= out_of;
+        x[u].load(table, (size_t)(out_of ? 0 : id[u]) * cols + c[u], cols - (int)c[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (v0 + u * 256u >= nvec) break;
+        float f[V];
+        x[u].take(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] *= scale;
+        const size_t off = (size_t)row[u] * cols + c[u];
+        const int n = cols - (int)c[u];
+        if (out_dtype == BF_F32) vec_store_n<float, V, AL>((float*)out + off, n, f);
+        else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)out + off, n, f);
+        else vec_store_n<f16_t, V, AL>((f16_t*)out + off, n, f);
+    }
+    if (bad && err_flag) atomicExch(err_flag, 1);
 }
 
 // ------------------------------------------------------------------ the sort: least significant digit first, stable
@@ -331,15 +339,38 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
 
 // ------------------------------------------------------------------ few tokens: one launch, no sort
 // A workgroup per token: the first token of its id gathers the others' places in order and sums their rows, each wave 64 V
-// columns and a share of the rows.
+// columns and a share of the rows.  Behind them, workgroups that write zeros into `zero_rows` rows each of a dense gradient,
+// where none of the tokens is.
+// Up to 512 tokens (x 1 024 fp32 columns, added into a gradient): 7 us with few repeats, 17 with half of them one token, 29
+// with all; the sort's launches take 22 from there on.  One workgroup draws some 80 GB/s, which is why not more.
 #define FEW 512
 template <typename T, int V, bool AL>
 __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restrict__ ids, int pad, int* __restrict__ err_flag,
-                                                        const SumArgs a) {
-    __shared__ unsigned long long words[FEW / 64];
+                                                                int zero_rows, const SumArgs a) {
+    constexpr int WAVES = FEW / 64;
+    __shared__ unsigned long long words[WAVES];
     __shared__ unsigned short list[FEW];
-    __shared__ float red[FEW / 64][64 * V];
+    __shared__ float red[WAVES][64 * V];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), me = blockIdx.x;
+    if (me >= a.n) {
+        const size_t row0 = (size_t)(me - a.n) * zero_rows;
+        const int rows = (int)min((size_t)zero_rows, a.vocab - row0);
+        list[tid] = 0;
+        __syncthreads();
+        if (tid < a.n) {
+            const int id = ids[tid];
+            const unsigned at = (unsigned)id - (unsigned)row0;
+            if (id >= 0 && id != pad && at < (unsigned)rows) list[at] = 1;
+        }
+        __syncthreads();
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r = wave; r < rows; r += WAVES) {
+            if (list[r]) continue;
+            float* g = a.grad + (row0 + r) * a.cols;
+            for (int c = lane * 4; c < a.cols; c += 256) vec_store_n<float, 4, AL>(g + c, a.cols - c, zero);
+        }
+        return;
+    }
     const int key = ids[me];
     if (key < 0 || key >= a.vocab) {
         if (tid == 0 && err_flag) atomicExch(err_flag, 1);
@@ -350,35 +381,33 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
     const unsigned long long votes = __ballot(same);
     if (lane == 0) words[wave] = votes;
     __syncthreads();
-    int rank = __popcll(votes & ((1ull << lane) - 1ull)), many = 0;
+    int many = 0;
     bool earlier = false;
 #pragma unroll
-    for (int w = 0; w < FEW / 64; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const unsigned long long v = words[w];
-        if (w < wave) rank += __popcll(v);
-        many += __popcll(v);
         const int below = me - w * 64;          // tokens of this word in front of this one
         earlier |= below >= 64 ? v != 0 : below > 0 ? (v & ((1ull << below) - 1ull)) != 0 : false;
+        if (w == wave && same) list[many + __popcll(v & ((1ull << lane) - 1ull))] = (unsigned short)tid;
+        many += __popcll(v);
     }
     if (earlier) return;                        // uniform: the first token of this id does the work
-    if (same) list[rank] = (unsigned short)tid;
     __syncthreads();
-    const int waves = FEW / 64;
-    const int shares = a.slabs >= waves ? 1 : waves / a.slabs;
-    for (int slab0 = 0; slab0 < a.slabs; slab0 += waves) {
+    const int shares = a.slabs >= WAVES ? 1 : WAVES / a.slabs;
+    for (int slab0 = 0; slab0 < a.slabs; slab0 += WAVES) {
         const int at = wave / shares, slab = slab0 + at, sh = wave - at * shares;
-        const bool in = slab < a.slabs && at < waves / shares;
+        const bool in = slab < a.slabs && at < WAVES / shares;
         const int per = (many + shares - 1) / shares, from = sh * per, to = in ? min(many, from + per) : 0;
         const int c = (slab * 64 + lane) * V, nc = a.cols - c;
         float acc[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = 0.f;
-        for (int t = from; t < to; t += 4) {
-            Chunk<T, V, AL> f[4];
+        for (int t = from; t < to; t += 8) {
+            Chunk<T, V, AL> f[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) f[u].load(a.dy, (size_t)list[min(t + u, to - 1)] * a.ld + c, nc);
+            for (int u = 0; u < 8; ++u) f[u].load(a.dy, (size_t)list[min(t + u, to - 1)] * a.ld + c, nc);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < 8; ++u) {
                 float v[V];
                 f[u].take(v);
 #pragma unroll
@@ -437,8 +466,11 @@ void embed_sum_launch(SumArgs a, hipStream_t s) {
 template <typename T, int V>
 void embed_bwd_type(bool few, bool al, const int32_t* ids, int pad, int* err_flag, const SumArgs& a, hipStream_t s) {
     if (few) {
-        if (al) hipLaunchKernelGGL((embed_few_kernel<T, V, true>), dim3((unsigned)a.n), dim3(FEW), 0, s, ids, pad, err_flag, a);
-        else hipLaunchKernelGGL((embed_few_kernel<T, V, false>), dim3((unsigned)a.n), dim3(FEW), 0, s, ids, pad, err_flag, a);
+        // some 64 KB a workgroup
+        const int zero_rows = a.cols >= 16384 ? 1 : 16384 / a.cols < FEW ? 16384 / a.cols : FEW;
+        const dim3 grid((unsigned)a.n + (a.accumulate ? 0u : (unsigned)(((size_t)a.vocab + zero_rows - 1) / zero_rows)));
+        if (al) hipLaunchKernelGGL((embed_few_kernel<T, V, true>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
+        else hipLaunchKernelGGL((embed_few_kernel<T, V, false>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
     } else if (al) {
         embed_sum_launch<T, V, true>(a, s);
     } else {
@@ -454,7 +486,7 @@ extern "C" int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int
     const char* name = "bf_embed_scaled_fwd";
     BF_REQUIRE(float_type(table_dtype) && float_type(out_dtype), BF_EINVAL, "%s: bad table_dtype %d or out_dtype %d", name,
                table_dtype, out_dtype);
-    BF_REQUIRE(n >= 0 && cols > 0 && vocab > 0, BF_EINVAL, "%s: bad shape (n=%d cols=%d vocab=%d)", name, n, cols, vocab);
+    BF_REQUIRE(n >= 0 && cols > 0 && cols <= (1 << 30) && vocab > 0, BF_EINVAL, "%s: bad shape (n=%d cols=%d vocab=%d)", name, n, cols, vocab);
     if (n == 0) return BF_OK;
     BF_REQUIRE(tokens && table && out, BF_EINVAL, "%s: null pointer", name);
     const size_t ts = bf_dtype_size(table_dtype), os = bf_dtype_size(out_dtype);
@@ -463,21 +495,26 @@ extern "C" int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int
     const int V = table_dtype == BF_F32 ? 4 : 8;
     const unsigned vpr = (unsigned)((cols + V - 1) / V);
     const unsigned long long nvec = (unsigned long long)n * vpr;
-    BF_REQUIRE(nvec <= 0xFFFFF000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
+    BF_REQUIRE(nvec <= 0x7FFFF000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
     const bool al = cols % V == 0 && bf_aligned16(table) && bf_aligned16(out);
-    const dim3 grid((unsigned)((nvec + 255) / 256)), block(256);
     hipStream_t s = (hipStream_t)stream;
+    // vectors a lane: many for a long batch (131 072 x 1 024 bf16: 75.9 us with four, 91.8 with one), one where the launch's
+    // latency counts (8 192 x 768: 5.9 us, with four 6.3; 77 x 512: 3.0 and 3.8)
+    const int U = nvec >= (1u << 21) ? 4 : 1;
+    const dim3 grid((unsigned)((nvec + 256 * U - 1) / (256 * U))), block(256);
+#define EMBED_FWD2(T, A, N)                                                                                                      \
+    hipLaunchKernelGGL((embed_scaled_kernel<T, A, N>), grid, block, 0, s, tokens, (const T*)table, out, out_dtype, scale,        \
+                       (unsigned)nvec, vpr, cols, vocab, err_flag)
 #define EMBED_FWD(T)                                                                                                             \
     do {                                                                                                                         \
-        if (al) hipLaunchKernelGGL((embed_scaled_kernel<T, true>), grid, block, 0, s, tokens, (const T*)table, out, out_dtype,   \
-                                   scale, (unsigned)nvec, vpr, cols, vocab, err_flag);                                           \
-        else hipLaunchKernelGGL((embed_scaled_kernel<T, false>), grid, block, 0, s, tokens, (const T*)table, out, out_dtype,     \
-                                scale, (unsigned)nvec, vpr, cols, vocab, err_flag);                                              \
+        if (al) { if (U == 4) EMBED_FWD2(T, true, 4); else EMBED_FWD2(T, true, 1); }                                             \
+        else { if (U == 4) EMBED_FWD2(T, false, 4); else EMBED_FWD2(T, false, 1); }                                              \
     } while (0)
     if (table_dtype == BF_F32) EMBED_FWD(float);
     else if (table_dtype == BF_BF16) EMBED_FWD(bf16_t);
     else EMBED_FWD(f16_t);
 #undef EMBED_FWD
+#undef EMBED_FWD2
     BF_CHECK_LAUNCH(name);
     return BF_OK;
 }
@@ -492,17 +529,18 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
                                    size_t workspace_bytes, bf_stream_t stream) {
     const char* name = "bf_embed_scaled_bwd";
     BF_REQUIRE(float_type(dy_dtype), BF_EINVAL, "%s: bad dy_dtype %d", name, dy_dtype);
-    BF_REQUIRE(n >= 0 && cols > 0 && vocab > 0 && vocab < 0x7FFFFFFF, BF_EINVAL, "%s: bad shape (n=%d cols=%d vocab=%d)", name, n,
+    BF_REQUIRE(n >= 0 && cols > 0 && cols <= (1 << 30) && vocab > 0 && vocab < 0x7FFFFFFF, BF_EINVAL, "%s: bad shape (n=%d cols=%d vocab=%d)", name, n,
                cols, vocab);
     BF_REQUIRE(n <= (1 << 30), BF_EINVAL, "%s: over 2^30 tokens (n=%d)", name, n);
     BF_REQUIRE(grad && (uintptr_t)grad % 4 == 0, BF_EALIGN, "%s: grad is null or not aligned to its element", name);
     hipStream_t s = (hipStream_t)stream;
-    if (n <= FEW && !accumulate) {
-        const size_t floats = (size_t)vocab * cols, blocks = (floats + 8191) / 8192;             // four 16-byte stores per thread
-        hipLaunchKernelGGL(embed_zero_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(512), 0, s, grad, floats);
-        BF_CHECK_LAUNCH(name);
+    if (n == 0) {
+        if (!accumulate) {
+            const hipError_t e = bf_zero_f32_async(grad, (size_t)vocab * cols, s);
+            BF_REQUIRE(e == hipSuccess, BF_ELAUNCH, "%s: launch failed", name);
+        }
+        return BF_OK;
     }
-    if (n == 0) return BF_OK;
     BF_REQUIRE(dy && tokens, BF_EINVAL, "%s: null pointer", name);
     BF_REQUIRE(ld_dy >= cols, BF_EINVAL, "%s: ld_dy=%lld is under cols=%d", name, (long long)ld_dy, cols);
     const size_t esz = bf_dtype_size(dy_dtype);
@@ -513,7 +551,9 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
     a.n = n; a.vocab = vocab; a.dy = dy; a.ld = ld_dy; a.cols = cols; a.scale = scale; a.accumulate = accumulate; a.grad = grad;
     a.slabs = (cols + 64 * V - 1) / (64 * V);
     const bool few = n <= FEW;
-    BF_REQUIRE((unsigned long long)n * a.slabs <= 0xFFFF0000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
+    // a grid counts threads in 32 bits: 2^24 workgroups of 256
+    BF_REQUIRE((unsigned long long)(n / 16 + 1) * a.slabs / 4 + (unsigned)vocab / 32 < (1u << 24) - 2, BF_EINVAL,
+               "%s: n=%d x cols=%d, vocab=%d is too large", name, n, cols, vocab);
     if (!few) {
         const EmbedPlan p = embed_plan(n, cols, vocab);
         BF_REQUIRE(workspace && workspace_bytes >= p.bytes, BF_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", name,

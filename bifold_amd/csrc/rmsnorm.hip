@@ -381,38 +381,40 @@ template <typename TDY>
 __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
     constexpr int V = 8;
     __shared__ float red[4];
-    const int row = blockIdx.x;
-    const TDY* dy = (const TDY*)a.dy + (size_t)row * a.ldy;
-    const float r = a.rstd[row];
-    auto chunk = [&](int c, float (&b)[V], float (&h)[V]) __attribute__((always_inline)) {
-        float g[V];
-        vec_load_n<TDY, V, false>(dy + c, a.cols - c, b);
-        vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
-        stream_load<V>(a, row, c, a.cols - c, h);
+    for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const TDY* dy = (const TDY*)a.dy + (size_t)row * a.ldy;
+        const float r = a.rstd[row];
+        auto chunk = [&](int c, float (&b)[V], float (&h)[V]) __attribute__((always_inline)) {
+            float g[V];
+            vec_load_n<TDY, V, false>(dy + c, a.cols - c, b);
+            vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
+            stream_load<V>(a, row, c, a.cols - c, h);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            b[j] *= g[j];
-            h[j] *= r;
+            for (int j = 0; j < V; ++j) {
+                b[j] *= g[j];
+                h[j] *= r;
+            }
+        };
+        float b[V], h[V], s = 0.f;
+        for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
+            chunk(c, b, h);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s = fmaf(b[j], h[j], s);
         }
-    };
-    float b[V], h[V], s = 0.f;
-    for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
-        chunk(c, b, h);
+        const float m = row_sum<4>(s, red) / (float)a.cols;
+        for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
+            chunk(c, b, h);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s = fmaf(b[j], h[j], s);
-    }
-    const float m = row_sum<4>(s, red) / (float)a.cols;
-    for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
-        chunk(c, b, h);
+            for (int j = 0; j < V; ++j) b[j] = r * (b[j] - h[j] * m);
+            if (a.dres) {
+                float d[V];
+                load_as<V, false>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, a.cols - c, d);
 #pragma unroll
-        for (int j = 0; j < V; ++j) b[j] = r * (b[j] - h[j] * m);
-        if (a.dres) {
-            float d[V];
-            load_as<V, false>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, a.cols - c, d);
-#pragma unroll
-            for (int j = 0; j < V; ++j) b[j] += d[j];
+                for (int j = 0; j < V; ++j) b[j] += d[j];
+            }
+            store_as<V, false>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, a.cols - c, b);
         }
-        store_as<V, false>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, a.cols - c, b);
+        __syncthreads();                        // red is written again
     }
 }
 // Launched in front of rms_bwd_long_kernel, which may write dx over dy.
@@ -457,6 +459,8 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
 
 // ------------------------------------------------------------------ dispatch
 #define RMS_LONG 8192                           /* widest row kept in the registers of one workgroup */
+#define RMS_SLICE (1 << 22)                     /* rows of one forward launch; a multiple of every alignment */
+#define RMS_MOST (1 << 30)                      /* rows, columns */
 
 template <typename TX, int V, bool AL> void rms_fwd_launch(const RmsFwd& a, hipStream_t s) {
     const dim3 wave((unsigned)((a.rows + 3) / 4)), wg((unsigned)a.rows), block(256);
@@ -524,7 +528,7 @@ template <typename TDY> void rms_bwd_any(const RmsBwd& a, bool al, hipStream_t s
     constexpr int dt = dtype_of<TDY>();
     if (rms_bwd_walks(dt, a.x_dtype, a.q != nullptr, a.dx_dtype, a.cols)) {
         hipLaunchKernelGGL((rms_dgamma_long_kernel<TDY>), dim3((unsigned)((a.cols + 255) / 256), (unsigned)a.nblk), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((rms_bwd_long_kernel<TDY>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((rms_bwd_long_kernel<TDY>), dim3((unsigned)(a.rows < RMS_SLICE ? a.rows : RMS_SLICE)), dim3(256), 0, s, a);
     } else if (a.dx_dtype == dt) {
         if (a.q) rms_bwd_types<TDY, Kept, TDY>(a, al, s);
         else if (a.x_dtype == dt) rms_bwd_types<TDY, TDY, TDY>(a, al, s);
@@ -546,7 +550,8 @@ bool any_float(int dt) { return dt == BF_F32 || bf_is_half(dt); }
 int rms_fwd(const char* name, RmsFwd& a, int x_dtype, bf_stream_t stream) {
     BF_REQUIRE(any_float(x_dtype), BF_EINVAL, "%s: bad x_dtype %d", name, x_dtype);
     BF_REQUIRE(!a.delta || any_float(a.d_dtype), BF_EINVAL, "%s: bad delta_dtype %d", name, a.d_dtype);
-    BF_REQUIRE(a.rows >= 0 && a.cols > 0, BF_EINVAL, "%s: bad shape (rows=%d cols=%d)", name, a.rows, a.cols);
+    BF_REQUIRE(a.rows >= 0 && a.rows <= RMS_MOST && a.cols > 0 && a.cols <= RMS_MOST, BF_EINVAL, "%s: bad shape (rows=%d cols=%d)",
+               name, a.rows, a.cols);
     BF_REQUIRE(a.ldx >= a.cols && (!a.delta || a.ldd >= a.cols) && (!a.x_out || a.ldo >= a.cols), BF_EINVAL,
                "%s: a leading dimension is under cols=%d", name, a.cols);
     BF_REQUIRE((a.q == nullptr) == (a.code == nullptr), BF_EINVAL, "%s: a checkpoint is q and code, or neither", name);
@@ -562,11 +567,27 @@ int rms_fwd(const char* name, RmsFwd& a, int x_dtype, bf_stream_t stream) {
     const bool al = a.cols % V == 0 && rows_aligned(a.x, a.ldx, xs, V) && rows_aligned(a.delta, a.ldd, ds, V) &&
                     rows_aligned(a.x_out, a.ldo, xs, V) && rows_aligned(a.y, a.cols, ys, V) && rows_aligned(a.q, a.cols, 1, V) &&
                     rows_aligned(a.gamma, a.cols, 4, V);
+    // a grid counts threads in 32 bits: very many rows are taken in slices
     hipStream_t s = (hipStream_t)stream;
-    if (x_dtype == BF_F32) rms_fwd_any<float>(a, al, s);
-    else if (x_dtype == BF_BF16) rms_fwd_any<bf16_t>(a, al, s);
-    else rms_fwd_any<f16_t>(a, al, s);
-    BF_CHECK_LAUNCH(name);
+    const int rows = a.rows;
+    for (int r0 = 0; r0 < rows; r0 += RMS_SLICE) {
+        RmsFwd b = a;
+        b.rows = rows - r0 < RMS_SLICE ? rows - r0 : RMS_SLICE;
+        b.x = (const char*)a.x + (size_t)r0 * a.ldx * xs;
+        if (a.delta) b.delta = (const char*)a.delta + (size_t)r0 * a.ldd * ds;
+        if (a.x_out) b.x_out = (char*)a.x_out + (size_t)r0 * a.ldo * xs;
+        b.y = (char*)a.y + (size_t)r0 * a.cols * ys;
+        if (a.y_scale) b.y_scale = a.y_scale + r0;
+        if (a.rstd) b.rstd = a.rstd + r0;
+        if (a.q) {
+            b.q = a.q + (size_t)r0 * a.cols;
+            b.code = a.code + (size_t)r0 * a.gpr;
+        }
+        if (x_dtype == BF_F32) rms_fwd_any<float>(b, al, s);
+        else if (x_dtype == BF_BF16) rms_fwd_any<bf16_t>(b, al, s);
+        else rms_fwd_any<f16_t>(b, al, s);
+        BF_CHECK_LAUNCH(name);
+    }
     return BF_OK;
 }
 
@@ -603,7 +624,8 @@ extern "C" int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const
                               void* dx, int dx_dtype, float* dgamma, float* parts_ws, int rows, int cols, bf_stream_t stream) {
     const char* name = "bf_rmsnorm_bwd";
     BF_REQUIRE(any_float(dy_dtype) && any_float(dx_dtype), BF_EINVAL, "%s: bad dy_dtype %d or dx_dtype %d", name, dy_dtype, dx_dtype);
-    BF_REQUIRE(rows >= 0 && cols > 0, BF_EINVAL, "%s: bad shape (rows=%d cols=%d)", name, rows, cols);
+    BF_REQUIRE(rows >= 0 && rows <= RMS_MOST && cols > 0 && cols <= RMS_MOST, BF_EINVAL, "%s: bad shape (rows=%d cols=%d)", name,
+               rows, cols);
     BF_REQUIRE((q == nullptr) == (code == nullptr), BF_EINVAL, "%s: a checkpoint is q and code, or neither", name);
     BF_REQUIRE(dgamma && (uintptr_t)dgamma % 4 == 0, BF_EINVAL, "%s: null dgamma", name);
     hipStream_t s = (hipStream_t)stream;

@@ -1084,12 +1084,19 @@ def _row_layout(t: torch.Tensor, name: str):
     if not shape or shape[-1] == 0:
         raise RuntimeError(f"{name} needs a last dimension of at least one element, got {tuple(shape)}")
     cols = shape[-1]
+    if cols > 1 << 30:
+        raise RuntimeError(f"{name} has rows of {cols} elements, 2^30 at most")
     if t.is_contiguous():
         return t.numel() // cols, cols, cols
     if len(shape) == 2 and (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or shape[0] == 1):
         return shape[0], cols, t.stride(0) if shape[0] > 1 else cols
     raise RuntimeError(f"{name} must be contiguous, or 2-D with unit inner stride and rows that do not overlap, got "
                        f"{tuple(shape)} {t.stride()}")
+
+
+def _few_rows(rows: int) -> None:
+    if rows > 1 << 30:
+        raise RuntimeError(f"{rows} rows, 2^30 at most")
 
 
 def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
@@ -1155,8 +1162,9 @@ def act8_unpack(kept: Checkpoint, dtype: torch.dtype, out: Optional[torch.Tensor
     q, code = _act8_parts(kept)
     if out is None:
         out = _like(q, dtype)
-    elif out.shape != q.shape or out.dtype != dtype:
-        raise RuntimeError(f"act8_unpack: out must be {dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+    elif out.shape != q.shape or out.dtype != dtype or _overlap(out, q) or _overlap(out, code):
+        raise RuntimeError(f"act8_unpack: out must be {dtype} {tuple(q.shape)} apart from the checkpoint, got {out.dtype} "
+                           f"{tuple(out.shape)}")
     rows, cols, ld = _row_layout(out, "out")
     check(lib.bf_act8_unpack(q.data_ptr(), code.data_ptr(), out.data_ptr(), ld, dtype_code(out), rows, cols,
                              _launch_stream(q, code, out)), "bf_act8_unpack")
@@ -1195,6 +1203,7 @@ def act8_gelu_bwd(dy: torch.Tensor, kept: Checkpoint, act: int, out: Optional[to
 # ----------------------------------------------------------------------------- RMS norm
 def _rms_args(x, gamma, delta, x_out, write_x):
     rows, cols, ldx = _row_layout(x, "x")
+    _few_rows(rows)
     _vector(gamma, cols, "gamma")
     ldd = d_dtype = ldo = 0
     if delta is None:
@@ -1259,6 +1268,7 @@ def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dg
     """dx = dres + d rmsnorm / dx (dy); dgamma_out [cols] is written.  `x`: the normed stream, a tensor or the checkpoint the
     forward left; rstd: the forward's.  dx has dres's dtype (dy's without one); `out` may be dres or dy."""
     rows, cols, ldy = _row_layout(dy, "dy")
+    _few_rows(rows)
     _vector(gamma, cols, "gamma"), _vector(rstd, rows, "rstd"), _vector(dgamma_out, cols, "dgamma_out")
     q = code = None
     ldx = x_dtype = ldr = 0
@@ -1297,7 +1307,9 @@ def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dg
 def _token_ids(tokens: torch.Tensor) -> int:
     if tokens.dtype != torch.int32 or not tokens.is_contiguous():
         raise TypeError(f"token ids must be a contiguous int32 tensor, got {tokens.dtype}")
-    return tokens.numel()
+    n = tokens.numel()
+    _few_rows(n)
+    return n
 
 
 def _flag(err_flag: Optional[torch.Tensor]) -> None:
@@ -1310,7 +1322,7 @@ def embed_scaled_fwd(tokens: torch.Tensor, table: torch.Tensor, scale: float, er
     """out [tokens, cols] = scale * table[token].  A token outside the table reads row 0 and sets err_flag."""
     n = _token_ids(tokens)
     _flag(err_flag)
-    if table.dim() != 2 or not table.is_contiguous() or 0 in table.shape:
+    if table.dim() != 2 or not table.is_contiguous() or 0 in table.shape or max(table.shape) >= 2 ** 31 - 1:
         raise RuntimeError(f"embed_scaled_fwd: table must be a contiguous [vocab, cols] tensor, got {tuple(table.shape)}")
     stream = _launch_stream(tokens, table, err_flag)
     vocab, cols = table.shape
@@ -1331,7 +1343,7 @@ def embed_scaled_bwd(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: 
     rows, cols, ld = _row_layout(dy, "dy")
     if rows != n:
         raise RuntimeError(f"embed_scaled_bwd: {rows} rows of dy for {n} tokens")
-    if vocab <= 0 or (padding_idx is not None and not 0 <= padding_idx < vocab):
+    if not 0 < vocab < 2 ** 31 - 1 or (padding_idx is not None and not 0 <= padding_idx < vocab):
         raise ValueError(f"embed_scaled_bwd: vocab={vocab}, padding_idx={padding_idx}")
     if out is None:
         if accumulate:

@@ -671,7 +671,7 @@ int bf_act8_gelu_bwd(const void* dy, int64_t ld_dy, const void* q, const void* c
 /* Root-mean-square norm with the residual's addition:  t = x + delta;  r = 1 / sqrt(mean(t^2) + eps);  y = t r gamma.
  *   x [rows, ldx] any float type; delta [rows, ld_delta] any float type or NULL; x_out [rows, ld_out] = t rounded to x's type,
  *   or NULL (may be x); y [rows, cols]; rstd [rows] = r, or NULL; q / code = the 8-bit checkpoint of t, or both NULL.
- *   t enters y, r and the checkpoint unrounded; statistics are fp32.
+ *   t enters y, r and the checkpoint unrounded; statistics are fp32.  rows, cols <= 2^30.  Outputs overlap no input but as said.
  * _fp8: y_fp8 = e4m3(y / row_scale), row_scale = max |y| / 448 per row (1 for a row of zeros, NaN for a row with a NaN or an
  *   infinity): bf_gemm_fp8's operand, as bf_layernorm_fwd_fp8 writes it.
  * bwd:  h = t r;  b = dy gamma;  dx = dres + r (b - h mean(b h));  dgamma [cols] = sum over rows of dy h (overwritten; summed
@@ -689,6 +689,7 @@ int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const void* x, i
                    int dx_dtype, float* dgamma, float* parts_ws, int rows, int cols, bf_stream_t stream);
 
 /* Embedding lookup with scaling, and the gradient of its table.
+ *   (n / 64 * ceil(cols / 256) + vocab / 32 < 2^24.)
  *   fwd: out [n, cols] = scale * table[tokens[i], :]  (table [vocab, cols]).  A token outside the table sets err_flag (may be
  *        NULL) and reads row 0, as bf_embed_tokens does.
  *   bwd: grad [vocab, cols] fp32 = scale * the sum of the rows of dy [n, ld_dy] that share the token; accumulate != 0 adds to

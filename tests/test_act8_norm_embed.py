@@ -86,7 +86,7 @@ def test_embedding_refusals(L):
     refused(L, lib.bf_embed_scaled_fwd(PTR + 2, PTR, L.F32, PTR, L.F32, 1.0, 4, 64, 100, None, None), -2, "aligned")
     refused(L, lib.bf_embed_scaled_fwd(PTR, PTR, L.F32, PTR, L.F32, 1.0, 1 << 30, 4096, 100, None, None), -1, "too large")
 
-    def bwd(dy=PTR, ld=64, dt=L.F16, ids=PTR, grad=PTR, n=1000, cols=64, vocab=100, ws=PTR, size=None, acc=1):
+    def bwd(dy=PTR, ld=64, dt=L.F16, ids=PTR, grad=PTR, n=2000, cols=64, vocab=100, ws=PTR, size=None, acc=1):
         size = lib.bf_embed_scaled_bwd_workspace_bytes(n, cols, vocab) if size is None else size
         return lib.bf_embed_scaled_bwd(dy, ld, dt, ids, grad, 1.0, acc, -1, n, cols, vocab, None, ws, size, None)
 

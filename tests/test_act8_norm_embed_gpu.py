@@ -402,7 +402,7 @@ def tokens_of(kind, n, vocab, g):
 
 
 EMBEDS = [(1, 1, 1), (1, 64, 100), (2, 7, 3), (77, 512, 49408), (300, 33, 1000), (511, 520, 50), (512, 1100, 300), (513, 16, 200),
-          (700, 1030, 513), (1000, 64, 1), (4096, 40, 32000), (5000, 768, 511), (9000, 24, 300000), (20000, 72, 65536), (70000, 8, 600),
+          (700, 1030, 513), (1000, 64, 1), (1024, 2100, 90), (1025, 520, 30), (1500, 7, 40), (4096, 40, 32000), (5000, 768, 511), (9000, 24, 300000), (20000, 72, 65536), (70000, 8, 600),
           (33000, 520, 20)]
 
 
@@ -508,6 +508,39 @@ def test_offsets_past_32_bits(ops, L, gpu):
     grad = ops.embed_scaled_bwd(torch.ones(800, cols, device=gpu), ids, vocab, 0.5)
     assert (grad[-1] == 200).all() and (grad[-2] == 100).all() and (grad[5] == 100).all()
     assert (grad[6:-2].abs().amax() == 0) and (grad[:5] == 0).all()
+
+
+def test_very_many_rows(ops, gpu):
+    """More rows than one launch takes: what lies at and behind the seam is what a call on those rows alone gives."""
+    rows, cols = (1 << 22) + 1000, 24
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(rows, cols, generator=g, device=gpu)
+    delta = torch.randn(rows, cols, generator=g, device=gpu).half()
+    gamma = torch.rand(cols, generator=g, device=gpu) + 0.5
+    part = slice((1 << 22) - 500, rows)
+    xo = torch.empty_like(x)
+    y, rstd, kept = ops.rmsnorm_fwd(x, gamma, torch.float16, delta=delta, x_out=xo, save_stats=True, checkpoint=True)
+    y8, scale, _, _ = ops.rmsnorm_fwd_fp8(x, gamma, delta=delta, write_x=False)
+    xo2 = torch.empty_like(x[part])
+    y2, r2, kept2 = ops.rmsnorm_fwd(x[part], gamma, torch.float16, delta=delta[part], x_out=xo2, save_stats=True, checkpoint=True)
+    y82, scale2, _, _ = ops.rmsnorm_fwd_fp8(x[part], gamma, delta=delta[part], write_x=False)
+    for a, b in ((y, y2), (rstd, r2), (kept[0], kept2[0]), (kept[1], kept2[1]), (xo, xo2), (y8, y82), (scale, scale2)):
+        assert torch.equal(a[part], b)
+    dg = torch.empty(cols, device=gpu)
+    for dy, stream in ((y, kept), (xo, xo.bfloat16())):                       # the second mixture takes the walking kernels
+        dx = ops.rmsnorm_bwd(dy, stream, gamma, rstd, dg)
+        cut = (stream[0][part], stream[1][part]) if isinstance(stream, tuple) else stream[part]
+        assert torch.equal(dx[part], ops.rmsnorm_bwd(dy[part], cut, gamma, rstd[part].clone(), torch.empty_like(dg)))
+        assert torch.isfinite(dg).all()
+
+
+def test_branch_that_is_the_stream(ops, gpu):
+    for cols in (64, 1500, 9000):
+        x = torch.randn(6, cols, device=gpu)
+        want, _, _ = ops.rmsnorm_fwd(x + x, torch.ones(cols, device=gpu), torch.float32)
+        double = x + x
+        got, _, _ = ops.rmsnorm_fwd(x, torch.ones(cols, device=gpu), torch.float32, delta=x)      # in place
+        assert torch.equal(got, want) and torch.equal(x, double)
 
 
 def step(ops, L, s):
