@@ -173,6 +173,96 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
     }
 }
 
+// Up to 2 048 tokens of a vocabulary under 2^18: the same sort by one workgroup, in LDS, one launch (the whole gradient of
+// 2 048 x 1 024 fp32, added into one that is there: 18 instead of 24 us; 4 096 tokens 24 and 28, 8 192 37 and 33: one CU is
+// not enough there).  A token is one word, its key over its place (11 bits; a larger
+// vocabulary would fit, but one workgroup also clears its table of bytes); a thread holds R of them, a wave R x 64
+// consecutive ones.  Places behind the last token hold the largest word, which stays behind.
+#define ONE_THREADS 1024
+#define ONE_WAVES 16
+#define ONE_BITS 11
+#define ONE_MAX (1 << ONE_BITS)
+#define ONE_BINS 256
+template <int R>
+__global__ __launch_bounds__(ONE_THREADS) void embed_sort_one_kernel(const SortArgs a, int passes) {
+    __shared__ unsigned buf[ONE_THREADS * R];
+    __shared__ int cnt[ONE_WAVES][ONE_BINS];
+    __shared__ int wave_tot[ONE_BINS / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int first = wave * 64 * R + lane, mask = (1 << a.dbits) - 1;
+    if (tid == 0) *a.owner_count = 0;
+    if (a.present) {
+        unsigned* words = (unsigned*)a.present;
+        const int many = (int)(((unsigned)a.vocab + 3u) >> 2);
+        for (int i = tid; i < many; i += ONE_THREADS) words[i] = 0;
+    }
+    unsigned item[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = first + r * 64;
+        item[r] = i < a.n ? (unsigned)sort_item<true>(a, i, a.err_flag).x << ONE_BITS | (unsigned)i : 0xFFFFFFFFu;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = ONE_BITS + pass * a.dbits;
+#pragma unroll
+        for (int k = 0; k < ONE_WAVES * ONE_BINS / ONE_THREADS; ++k) (&cnt[0][0])[k * ONE_THREADS + tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) atomicAdd(&cnt[wave][(item[r] >> shift) & mask], 1);
+        __syncthreads();
+        int tot = 0, scan = 0;
+        if (tid < ONE_BINS) {
+#pragma unroll
+            for (int w = 0; w < ONE_WAVES; ++w) tot += cnt[w][tid];
+            scan = tot;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int up = __shfl_up(scan, o, 64);
+                if (lane >= o) scan += up;
+            }
+            if (lane == 63) wave_tot[wave] = scan;
+        }
+        __syncthreads();
+        if (tid < ONE_BINS) {
+            for (int w = 0; w < wave; ++w) scan += wave_tot[w];
+            int place = scan - tot;
+#pragma unroll
+            for (int w = 0; w < ONE_WAVES; ++w) {
+                const int c = cnt[w][tid];
+                cnt[w][tid] = place;
+                place += c;
+            }
+        }
+        __syncthreads();
+        int* mine = cnt[wave];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int d = (item[r] >> shift) & mask;
+            unsigned long long same = ~0ull;
+            for (int b = 0; b < a.dbits; ++b) {
+                const bool bit = (d >> b) & 1;
+                const unsigned long long votes = __ballot(bit);
+                same &= bit ? votes : ~votes;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1ull));
+            const int at = __hip_atomic_load(&mine[d], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            buf[at + rank] = item[r];
+            if (rank == 0) __hip_atomic_store(&mine[d], at + __popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) item[r] = buf[first + r * 64];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = first + r * 64, key = (int)(item[r] >> ONE_BITS);
+        if (i < a.n) {
+            a.out[i] = make_int2(key, (int)(item[r] & (ONE_MAX - 1)));
+            if (a.present && key < a.vocab) a.present[key] = 1;
+        }
+    }
+}
+
 // ------------------------------------------------------------------ sums over runs of equal keys
 struct SumArgs {
     const int2* sorted; int n; int vocab; int chunk, chunks, slabs;        // (key, row of dy), by key, then row
@@ -431,6 +521,7 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
 
 // ------------------------------------------------------------------ plan of a call
 struct EmbedPlan {
+    bool one;                                   // sorted by one workgroup
     int passes, dbits, rounds, tiles, chunk, chunks;
     size_t pairs, hist, owners, present, part, bytes;            // offsets into the workspace
 };
@@ -438,7 +529,8 @@ EmbedPlan embed_plan(int n, int cols, int vocab) {
     EmbedPlan p;
     int bits = 0;
     while (bits < 31 && (vocab >> bits) != 0) ++bits;            // the key `vocab` itself is used
-    p.passes = (bits + 8) / 9;
+    p.one = n <= ONE_MAX && vocab < (1 << 18);
+    p.passes = p.one ? (bits + 7) / 8 : (bits + 8) / 9;          // digits of up to 8 or 9 bits
     p.dbits = (bits + p.passes - 1) / p.passes;
     const long span = (long)SORT_THREADS * SORT_MAX_TILES;
     p.rounds = (int)((n + span - 1) / span);
@@ -566,8 +658,15 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
         q.ids = tokens; q.n = n; q.vocab = vocab; q.pad = padding_idx; q.hist = (int*)(ws + p.hist);
         q.owner_count = (int*)(owners + p.chunks); q.err_flag = err_flag; q.rounds = p.rounds; q.tiles = p.tiles; q.dbits = p.dbits;
         q.present = accumulate ? nullptr : (uint8_t*)(ws + p.present);
+        if (p.one) {
+            q.out = pairs[0];
+            const dim3 block(ONE_THREADS);
+            if (n <= 1024) hipLaunchKernelGGL(embed_sort_one_kernel<1>, dim3(1), block, 0, s, q, p.passes);
+            else hipLaunchKernelGGL(embed_sort_one_kernel<2>, dim3(1), block, 0, s, q, p.passes);
+            BF_CHECK_LAUNCH(name);
+        }
         const dim3 grid((unsigned)p.tiles), block(SORT_THREADS);
-        for (int pass = 0; pass < p.passes; ++pass) {
+        for (int pass = 0; pass < p.passes && !p.one; ++pass) {
             q.shift = pass * p.dbits;
             q.in = pairs[(pass + 1) & 1];
             q.out = pairs[pass & 1];
