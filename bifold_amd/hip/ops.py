@@ -1099,25 +1099,27 @@ def _few_rows(rows: int) -> None:
         raise RuntimeError(f"{rows} rows, 2^30 at most")
 
 
+def _leading(t: torch.Tensor, cols: int, name: str) -> int:
+    """Leading dimension of a tensor whose shape has been looked at."""
+    return cols if t.is_contiguous() else _row_layout(t, name)[2]
+
+
 def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
     return t
 
 
-def _span(t: torch.Tensor):
-    at = t.data_ptr()
-    if t.is_contiguous():
-        return at, at + t.numel() * t.element_size()
-    return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do the address ranges of two tensors meet?  (Strided views count from their first to their last element.)"""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if a.is_contiguous() and b.is_contiguous():
+        na, nb = a.nbytes, b.nbytes
+    else:
+        if a.numel() == 0 or b.numel() == 0:
+            return False
+        na, nb = ((sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b))
+    return pa < pb + nb and pb < pa + na and na > 0 and nb > 0
 
 
 def _apart_or_same(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1134,7 +1136,7 @@ Checkpoint = Tuple[torch.Tensor, torch.Tensor]
 
 def _act8_empty(x: torch.Tensor) -> Checkpoint:
     shape = x.shape
-    return _like(x, torch.int8), x.new_empty((*shape[:-1], (shape[-1] + ACT8_GROUP - 1) // ACT8_GROUP), dtype=torch.uint8)
+    return _like(x, torch.int8), x.new_empty(*shape[:-1], (shape[-1] + ACT8_GROUP - 1) // ACT8_GROUP, dtype=torch.uint8)
 
 
 def _act8_parts(kept: Checkpoint):
@@ -1194,7 +1196,7 @@ def act8_gelu_bwd(dy: torch.Tensor, kept: Checkpoint, act: int, out: Optional[to
     elif out.shape != dy.shape or out.dtype != dy.dtype or not _apart_or_same(out, dy) or _overlap(out, q) or _overlap(out, code):
         raise RuntimeError("act8_gelu_bwd: out has dy's shape and dtype, and is dy or memory of its own")
     else:
-        _, _, ldo = _row_layout(out, "out")
+        ldo = _leading(out, cols, "out")
     check(lib.bf_act8_gelu_bwd(dy.data_ptr(), ld, q.data_ptr(), code.data_ptr(), out.data_ptr(), ldo, dtype_code(dy), act, rows,
                                cols, _launch_stream(dy, q, code, out)), "bf_act8_gelu_bwd")
     return out
@@ -1213,7 +1215,7 @@ def _rms_args(x, gamma, delta, x_out, write_x):
     else:
         if delta.shape != x.shape:
             raise RuntimeError(f"rmsnorm: delta {tuple(delta.shape)} does not match x {tuple(x.shape)}")
-        _, _, ldd = _row_layout(delta, "delta")
+        ldd = _leading(delta, cols, "delta")
         d_dtype = dtype_code(delta)
         if not write_x:
             x_out = None
@@ -1225,7 +1227,7 @@ def _rms_args(x, gamma, delta, x_out, write_x):
                     raise RuntimeError("rmsnorm: x_out has x's shape and dtype")
                 if not _apart_or_same(x_out, x):
                     raise RuntimeError("rmsnorm: x_out is x or memory of its own")
-                _, _, ldo = _row_layout(x_out, "x_out")
+                ldo = _leading(x_out, cols, "x_out")
             if not _apart_or_same(x_out, delta):
                 raise RuntimeError("rmsnorm: x_out is delta or memory of its own")
     return rows, cols, ldx, ldd, d_dtype, ldo, x_out, _launch_stream(x, gamma, delta, x_out)
@@ -1283,7 +1285,7 @@ def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dg
         raise RuntimeError(f"rmsnorm_bwd: dy {tuple(dy.shape)}, x {tuple(shape)} and dres must have one shape")
     dt = dy.dtype if dres is None else dres.dtype
     if dres is not None:
-        _, _, ldr = _row_layout(dres, "dres")
+        ldr = _leading(dres, cols, "dres")
     if out is None:
         out = _like(dy, dt)
     else:
