@@ -13,100 +13,103 @@
 
 #define ACT8_GROUP 32
 
-// V consecutive elements as fp32.  AL: the address is aligned to the vector (at most 16 bytes); otherwise only to the element
-// -- global memory takes unaligned 16-byte accesses on this target, so an odd width costs split cache lines and no scalar path.
-template <typename T, int V, bool AL>
-__device__ __forceinline__ void vec_load(const T* p, float (&o)[V]) {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    vec r;
-    constexpr int A = sizeof(vec) < 16 ? sizeof(vec) : 16;
-    if constexpr (AL) __builtin_memcpy(&r, __builtin_assume_aligned(p, A), sizeof(vec));
-    else __builtin_memcpy(&r, p, sizeof(vec));
+// How a kernel reads rows in vectors of V elements.  ALIGNED: rows begin at addresses aligned to a vector (at most 16 bytes)
+// and hold whole vectors.  ANY: rows of at least V elements anywhere; the vector at a row's end is read V elements in front
+// of the end -- global memory takes unaligned 16-byte accesses on this target -- and moved down in registers, so an odd width
+// costs split cache lines and some vector instructions, but no branch and no element-wise loads (20 000 x 1 155 bf16, RMS
+// norm backward: 43 us, element by element 57).  TINY: shorter rows, element by element.
+enum { ROWS_TINY = 0, ROWS_ANY = 1, ROWS_ALIGNED = 2 };
+
+// w moved down by `bytes` (0 .. 4 W), zeros from above; `bytes` may differ from lane to lane
+template <int W> __device__ __forceinline__ void shift_down(unsigned (&w)[W], int bytes) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = to_f32<T>(r[j]);
-}
-template <typename T, int V, bool AL>
-__device__ __forceinline__ void vec_store(T* p, const float (&v)[V]) {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    vec r;
+    for (int step = W; step >= 1; step >>= 1) {                // words
+        const bool by = bytes & (4 * step);
 #pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = from_f32<T>(v[j]);
-    constexpr int A = sizeof(vec) < 16 ? sizeof(vec) : 16;
-    if constexpr (AL) __builtin_memcpy(__builtin_assume_aligned(p, A), &r, sizeof(vec));
-    else __builtin_memcpy(p, &r, sizeof(vec));
-}
-// the same with only n of the V elements there (n <= 0: none); the others read as zero and are not written.  With AL a
-// vector is there as a whole or not at all.
-template <typename T, int V, bool AL>
-__device__ __forceinline__ void vec_load_n(const T* p, int n, float (&o)[V]) {
-    if (n >= V) {
-        vec_load<T, V, AL>(p, o);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = !AL && j < n ? to_f32<T>(p[j]) : 0.f;
+        for (int k = 0; k < W; ++k) w[k] = by ? (k + step < W ? w[k + step] : 0u) : w[k];
     }
-}
-template <typename T, int V, bool AL>
-__device__ __forceinline__ void vec_store_n(T* p, int n, const float (&v)[V]) {
-    if (n >= V) {
-        vec_store<T, V, AL>(p, v);
-    } else if constexpr (!AL) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < n) p[j] = from_f32<T>(v[j]);
-    }
+    for (int k = 0; k < W; ++k) w[k] = __builtin_amdgcn_alignbyte(k + 1 < W ? w[k + 1] : 0u, w[k], (unsigned)bytes & 3u);
 }
-// V elements as they lie in memory: nothing waits for the load until the values are taken (a conversion behind each of several
-// loads, as a branch on a run-time type or bound makes it, waits for one after the other).
-template <typename T, int V, bool AL> struct Chunk {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    vec r;
+
+// V elements of a row as they lie in memory, n of them (<= 0: none) in front of the row's end.  Nothing waits for the load
+// until the values are taken: a conversion behind each of several loads, as a branch on a run-time type makes it, waits for
+// one after the other.
+template <typename T, int V, int A> struct Chunk {
+    static constexpr int W = V * (int)sizeof(T) / 4;
+    unsigned w[W];
     __device__ __forceinline__ void load(const void* base, size_t off, int n) {
         const T* p = (const T*)base + off;
-        if (n >= V) {
-            constexpr int A = sizeof(vec) < 16 ? sizeof(vec) : 16;
-            if constexpr (AL) __builtin_memcpy(&r, __builtin_assume_aligned(p, A), sizeof(vec));
-            else __builtin_memcpy(&r, p, sizeof(vec));
-        } else {
+        if constexpr (A == ROWS_ANY) {
+            __builtin_memcpy(w, p + min(0, n - V), sizeof(w));
+        } else if constexpr (A == ROWS_ALIGNED) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) r[j] = !AL && j < n ? p[j] : from_f32<T>(0.f);
+            for (int k = 0; k < W; ++k) w[k] = 0;
+            if (n >= V) __builtin_memcpy(w, __builtin_assume_aligned(p, sizeof(w) < 16 ? sizeof(w) : 16), sizeof(w));
+        } else {
+            T t[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                t[j] = T(0);
+                if (j < n) t[j] = p[j];
+            }
+            __builtin_memcpy(w, t, sizeof(w));
         }
     }
-    __device__ __forceinline__ void take(float (&o)[V]) const {
+    // the words, zeros behind the row's end
+    __device__ __forceinline__ void words(unsigned (&o)[W], int n) const {
+#pragma unroll
+        for (int k = 0; k < W; ++k) o[k] = w[k];
+        if constexpr (A == ROWS_ANY) shift_down<W>(o, (V - max(0, min(n, V))) * (int)sizeof(T));
+    }
+    __device__ __forceinline__ void take(float (&o)[V], int n) const {
+        typedef T vec __attribute__((ext_vector_type(V)));
+        unsigned u[W];
+        words(u, n);
+        vec r;
+        __builtin_memcpy(&r, u, sizeof(u));
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = to_f32<T>(r[j]);
     }
     // The load is complete behind this point.  (Stores count in vmcnt too: a wait that the compiler places between stores
     // which may or may not happen is a wait for those stores.)
-    __device__ __forceinline__ void arrived() { asm volatile("" : "+v"(r)); }
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int k = 0; k < W; ++k) asm volatile("" : "+v"(w[k]));
+    }
 };
-// the wave's number in its workgroup, as the scalar it is: rows, tokens and branches that depend on it stay scalar too
-__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
-// V bytes <-> V / 4 words
-template <int V, bool AL>
-__device__ __forceinline__ void bytes_store_n(uint8_t* p, int n, const unsigned (&w)[V / 4]) {
+template <typename T, int V, int A> __device__ __forceinline__ void vec_load_n(const T* p, int n, float (&o)[V]) {
+    Chunk<T, V, A> c;
+    c.load(p, 0, n);
+    c.take(o, n);
+}
+template <typename T, int V, int A> __device__ __forceinline__ void vec_store_n(T* p, int n, const float (&v)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r[j] = from_f32<T>(v[j]);
     if (n >= V) {
-        if constexpr (AL) __builtin_memcpy(__builtin_assume_aligned(p, V), w, V);
+        if constexpr (A == ROWS_ALIGNED) __builtin_memcpy(__builtin_assume_aligned(p, sizeof(r) < 16 ? sizeof(r) : 16), &r, sizeof(r));
+        else __builtin_memcpy(p, &r, sizeof(r));
+    } else if constexpr (A != ROWS_ALIGNED) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n) p[j] = r[j];
+    }
+}
+// V bytes from V / 4 words
+template <int V, int A> __device__ __forceinline__ void bytes_store_n(uint8_t* p, int n, const unsigned (&w)[V / 4]) {
+    if (n >= V) {
+        if constexpr (A == ROWS_ALIGNED) __builtin_memcpy(__builtin_assume_aligned(p, V), w, V);
         else __builtin_memcpy(p, w, V);
-    } else if constexpr (!AL) {
+    } else if constexpr (A != ROWS_ALIGNED) {
 #pragma unroll
         for (int j = 0; j < V; ++j)
             if (j < n) p[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
     }
 }
-template <int V, bool AL>
-__device__ __forceinline__ void bytes_load_n(const uint8_t* p, int n, unsigned (&w)[V / 4]) {
-    if (n >= V) {
-        if constexpr (AL) __builtin_memcpy(w, __builtin_assume_aligned(p, V), V);
-        else __builtin_memcpy(w, p, V);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V / 4; ++j) w[j] = 0;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (!AL && j < n) w[j >> 2] |= (unsigned)p[j] << (8 * (j & 3));
-    }
-}
+// the wave's number in its workgroup, as the scalar it is: rows, tokens and branches that depend on it stay scalar too
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
 // Largest magnitude of V elements as the bits of a non-negative float: an integer maximum, so a NaN (whose bits lie above
 // infinity's) is kept where fmaxf would drop it.

@@ -56,55 +56,60 @@ struct A8Args {
     unsigned nvec; unsigned vpr; int cols; int gpr;
 };
 
-template <typename T, int MODE, int ACT, bool DENSE, int V>
+template <typename T, int MODE, int ACT, int A, int V>
 __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
     constexpr bool EXACT = sizeof(T) == 4;
     constexpr unsigned PER = ACT8_GROUP / V;                   // lanes per group
     const unsigned v = blockIdx.x * 256u + threadIdx.x;
-    int n = v < a.nvec ? V : 0;
+    const bool live = v < a.nvec;
+    int n;                                                     // elements of the row from here on (at most V; <= 0: behind it)
     size_t off_x, off_y, off_q, off_c;
     bool first;
-    if constexpr (DENSE) {
+    if constexpr (A == ROWS_ALIGNED) {
+        n = live ? V : 0;
         off_x = off_y = off_q = (size_t)v * V;
         off_c = v / PER;
-        first = v % PER == 0 && n > 0;
-    } else {
-        const unsigned row = v / a.vpr, c = (v - row * a.vpr) * V;
-        if (n) n = min(V, a.cols - (int)c);                    // <= 0 in the lanes that fill up the row's last group
+        first = v % PER == 0;
+    } else {                                                   // lanes behind the last vector read it again
+        const unsigned w = min(v, a.nvec - 1), row = w / a.vpr, c = (w - row * a.vpr) * V;
+        n = min(V, a.cols - (int)c);
         off_x = (size_t)row * a.ldx + c;
         off_y = (size_t)row * a.ldy + c;
         off_q = (size_t)row * a.cols + c;
         off_c = (size_t)row * a.gpr + c / ACT8_GROUP;
-        first = c % ACT8_GROUP == 0 && n > 0;
+        first = c % ACT8_GROUP == 0;
     }
+    const int put = live ? n : 0;                              // elements to write
     const T* x = (const T*)a.x + off_x;
     T* y = (T*)a.y + off_y;
     float f[V];
     unsigned w[V / 4], code;
     if constexpr (MODE == A8_PACK || MODE == A8_FWD) {
-        vec_load_n<T, V, DENSE>(x, n, f);
+        vec_load_n<T, V, A>(x, n, f);
         code = act8_code(group_max<V>(magnitude_bits<V>(f)));
         act8_quant<V>(f, code, w);
-        bytes_store_n<V, DENSE>(a.q + off_q, n, w);
-        if (first) a.code[off_c] = (uint8_t)code;
+        bytes_store_n<V, A>(a.q + off_q, put, w);
+        if (first && put > 0) a.code[off_c] = (uint8_t)code;
         if constexpr (MODE == A8_FWD) {
 #pragma unroll
             for (int j = 0; j < V; ++j) f[j] = act_value<ACT, EXACT>(f[j]);
-            vec_store_n<T, V, DENSE>(y, n, f);
+            vec_store_n<T, V, A>(y, put, f);
         }
     } else {
-        Chunk<T, V, DENSE> dy;
-        bytes_load_n<V, DENSE>(a.q + off_q, n, w);
+        Chunk<T, V, A> dy;
+        Chunk<uint8_t, V, A> q;
+        q.load(a.q, off_q, n);
         code = n > 0 ? a.code[off_c] : 1u;
         if constexpr (MODE == A8_BWD) dy.load(x, 0, n);
+        q.words(w, n);
         act8_dequant<V>(w, code, f);
         if constexpr (MODE == A8_BWD) {
             float d[V];
-            dy.take(d);
+            dy.take(d, n);
 #pragma unroll
             for (int j = 0; j < V; ++j) f[j] = d[j] * act_slope<ACT, EXACT>(f[j]);
         }
-        vec_store_n<T, V, DENSE>(y, n, f);
+        vec_store_n<T, V, A>(y, put, f);
     }
 }
 
@@ -116,9 +121,11 @@ void act8_launch(const A8Args& a, bool dense, hipStream_t s) {
         constexpr int V = sizeof(T) == 4 && MODE != A8_UNPACK ? 4 : 8;
         A8Args b = a;
         b.nvec = a.nvec * (8 / V);
-        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, true, V>), dim3((unsigned)(((size_t)b.nvec + 255) / 256)), dim3(256), 0, s, b);
+        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, ROWS_ALIGNED, V>), dim3((unsigned)(((size_t)b.nvec + 255) / 256)), dim3(256), 0, s, b);
     } else {
-        hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, false, 8>), dim3((unsigned)(((size_t)a.nvec + 255) / 256)), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)(((size_t)a.nvec + 255) / 256));
+        if (a.cols >= 8) hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, ROWS_ANY, 8>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((act8_kernel<T, MODE, ACT, ROWS_TINY, 8>), grid, dim3(256), 0, s, a);
     }
 }
 

@@ -11,7 +11,7 @@
 namespace {
 
 // ------------------------------------------------------------------ lookup
-template <typename TT, bool AL, int U>
+template <typename TT, int A, int U>
 __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __restrict__ ids, const TT* __restrict__ table,
                                                            void* __restrict__ out, int out_dtype, float scale, unsigned nvec,
                                                            unsigned vpr, int cols, int vocab, int* __restrict__ err_flag) {
@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
     // two dependent loads: all ids first, then all rows, no branch between (which would wait for each)
     unsigned row[U], c[U];
     int id[U];
-    Chunk<TT, V, AL> x[U];
+    Chunk<TT, V, A> x[U];
     const unsigned v0 = blockIdx.x * (256u * U) + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -39,14 +39,14 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
     for (int u = 0; u < U; ++u) {
         if (v0 + u * 256u >= nvec) break;
         float f[V];
-        x[u].take(f);
+        const int n = cols - (int)c[u];
+        x[u].take(f, n);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] *= scale;
         const size_t off = (size_t)row[u] * cols + c[u];
-        const int n = cols - (int)c[u];
-        if (out_dtype == BF_F32) vec_store_n<float, V, AL>((float*)out + off, n, f);
-        else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)out + off, n, f);
-        else vec_store_n<f16_t, V, AL>((f16_t*)out + off, n, f);
+        if (out_dtype == BF_F32) vec_store_n<float, V, A>((float*)out + off, n, f);
+        else if (out_dtype == BF_BF16) vec_store_n<bf16_t, V, A>((bf16_t*)out + off, n, f);
+        else vec_store_n<f16_t, V, A>((f16_t*)out + off, n, f);
     }
     if (bad && err_flag) atomicExch(err_flag, 1);
 }
@@ -270,14 +270,14 @@ struct SumArgs {
     float* grad; float* part; int2* owners; int* owner_count;              // owners: (chunk, key) of each cut run
     const uint8_t* present; unsigned sum_blocks;                 // present: NULL, or the other rows' zeros are written too
 };
-template <int V, bool AL>
+template <int V, int A>
 __device__ __forceinline__ void grad_write(const SumArgs& a, int key, int c, const float (&acc)[V]) {
     float* g = a.grad + (size_t)key * a.cols + c;
     float o[V];
-    if (a.accumulate) vec_load_n<float, V, AL>(g, a.cols - c, o);
+    if (a.accumulate) vec_load_n<float, V, A>(g, a.cols - c, o);
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = a.accumulate ? o[j] + acc[j] * a.scale : acc[j] * a.scale;
-    vec_store_n<float, V, AL>(g, a.cols - c, o);
+    vec_store_n<float, V, A>(g, a.cols - c, o);
 }
 // One wave takes `chunk` (at most 64) consecutive sorted tokens and 64 V columns, eight rows in flight.  A run of equal keys
 // belongs to the chunk it begins in, which follows it into the next chunk.  Only a run that covers a whole further chunk is
@@ -287,7 +287,7 @@ __device__ __forceinline__ void grad_write(const SumArgs& a, int key, int c, con
 // arrived before its sums begin: with a wait per row, stores of finished runs between them were waited for too.
 // 131 072 x 1 024 bf16, vocabulary 65 536, 61 000 rows alive: 93 us for some 400 MB, 4.3 TB/s; 8 192 x 768 fp16, 32 000:
 // 18.5 us for 111 MB, 6.0 TB/s.
-template <typename T, int V, bool AL>
+template <typename T, int V, int A>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
     const int lane = threadIdx.x & 63;
     if (blockIdx.x >= a.sum_blocks) {           // a wave per eight rows of the table
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
         for (int r = 0; r < rows; ++r) {
             if ((there >> r) & 1) continue;
             float* g = a.grad + (row0 + r) * a.cols;
-            for (int c = lane * 4; c < a.cols; c += 256) vec_store_n<float, 4, AL>(g + c, a.cols - c, zero);
+            for (int c = lane * 4; c < a.cols; c += 256) vec_store_n<float, 4, A>(g + c, a.cols - c, zero);
         }
         return;
     }
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
     while (i < stop) {
-        Chunk<T, V, AL> f[8];
+        Chunk<T, V, A> f[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int at = min(i + u, stop - 1);
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
             if (i + u < stop) {
                 const int at = i + u;
                 float v[V];
-                f[u].take(v);
+                f[u].take(v, nc);
 #pragma unroll
                 for (int j = 0; j < V; ++j) acc[j] += v[j];
                 const int key = at < here ? __builtin_amdgcn_readlane(kl, at) : k_last;
@@ -358,12 +358,12 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
                 const int after = at + 1 == stop ? -1 : at + 1 < here ? __builtin_amdgcn_readlane(kl, at + 1) : k_last;
                 if (after != key) {
                     if (head) {
-                        vec_store_n<float, V, AL>(part, nc, acc);
+                        vec_store_n<float, V, A>(part, nc, acc);
                     } else if (cut && at + 1 == stop) {
-                        vec_store_n<float, V, AL>(part + a.cols, nc, acc);
+                        vec_store_n<float, V, A>(part + a.cols, nc, acc);
                         if (slab == 0 && lane == 0) a.owners[atomicAdd(a.owner_count, 1)] = make_int2(chunk, key);
                     } else {
-                        grad_write<V, AL>(a, key, c, acc);
+                        grad_write<V, A>(a, key, c, acc);
                     }
                     head = false;
 #pragma unroll
@@ -376,6 +376,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
 }
 // One workgroup per cut run (their order in the list does not matter: each has a gradient row of its own) and 256 columns:
 // finds the last chunk that starts with the run's key, sums the partial rows in order, sixteen waves a share each.
+template <int A>
 __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
     __shared__ float4 red[16][64];
     __shared__ int found[16];
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
         const int from = wave * share, to = min(many, from + share);
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
         for (int t = from; t < to; t += 8) {
-            Chunk<float, 4, false> f[8];
+            Chunk<float, 4, A> f[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int at = min(t + u, to - 1);
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 float v[4];
-                f[u].take(v);
+                f[u].take(v, nc);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[j] += t + u < to ? v[j] : 0.f;
             }
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
                 const float4 f = red[k][lane];
                 acc[0] += f.x; acc[1] += f.y; acc[2] += f.z; acc[3] += f.w;
             }
-            grad_write<4, false>(a, key, c, acc);
+            grad_write<4, A>(a, key, c, acc);
         }
         __syncthreads();
     }
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const SumArgs a) {
 // Up to 512 tokens (x 1 024 fp32 columns, added into a gradient): 7 us with few repeats, 17 with half of them one token, 29
 // with all; the sort's launches take 22 from there on.  One workgroup draws some 80 GB/s, which is why not more.
 #define FEW 512
-template <typename T, int V, bool AL>
+template <typename T, int V, int A>
 __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restrict__ ids, int pad, int* __restrict__ err_flag,
                                                                 int zero_rows, const SumArgs a) {
     constexpr int WAVES = FEW / 64;
@@ -461,7 +462,7 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
         for (int r = wave; r < rows; r += WAVES) {
             if (list[r]) continue;
             float* g = a.grad + (row0 + r) * a.cols;
-            for (int c = lane * 4; c < a.cols; c += 256) vec_store_n<float, 4, AL>(g + c, a.cols - c, zero);
+            for (int c = lane * 4; c < a.cols; c += 256) vec_store_n<float, 4, A>(g + c, a.cols - c, zero);
         }
         return;
     }
@@ -497,13 +498,13 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = 0.f;
         for (int t = from; t < to; t += 8) {
-            Chunk<T, V, AL> f[8];
+            Chunk<T, V, A> f[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) f[u].load(a.dy, (size_t)list[min(t + u, to - 1)] * a.ld + c, nc);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 float v[V];
-                f[u].take(v);
+                f[u].take(v, nc);
 #pragma unroll
                 for (int j = 0; j < V; ++j) acc[j] += t + u < to ? v[j] : 0.f;
             }
@@ -519,7 +520,7 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
             }
             __syncthreads();
         }
-        if (sh == 0 && in) grad_write<V, AL>(a, key, c, acc);
+        if (sh == 0 && in) grad_write<V, A>(a, key, c, acc);
     }
 }
 
@@ -553,26 +554,33 @@ EmbedPlan embed_plan(int n, int cols, int vocab) {
     return p;
 }
 
-template <typename T, int V, bool AL>
+template <typename T, int V, int A>
 void embed_sum_launch(SumArgs a, hipStream_t s) {
     a.sum_blocks = (unsigned)(((size_t)a.chunks * a.slabs + 3) / 4);
     const unsigned zeros = a.present ? (unsigned)(((size_t)a.vocab + 31) / 32) : 0u;
-    hipLaunchKernelGGL((embed_sum_kernel<T, V, AL>), dim3(a.sum_blocks + zeros), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((embed_sum_kernel<T, V, A>), dim3(a.sum_blocks + zeros), dim3(256), 0, s, a);
 }
 template <typename T, int V>
-void embed_bwd_type(bool few, bool al, const int32_t* ids, int pad, int* err_flag, const SumArgs& a, hipStream_t s) {
+void embed_bwd_type(bool few, int mode, const int32_t* ids, int pad, int* err_flag, const SumArgs& a, hipStream_t s) {
     if (few) {
         // some 64 KB a workgroup
         const int zero_rows = a.cols >= 16384 ? 1 : 16384 / a.cols < FEW ? 16384 / a.cols : FEW;
         const dim3 grid((unsigned)a.n + (a.accumulate ? 0u : (unsigned)(((size_t)a.vocab + zero_rows - 1) / zero_rows)));
-        if (al) hipLaunchKernelGGL((embed_few_kernel<T, V, true>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
-        else hipLaunchKernelGGL((embed_few_kernel<T, V, false>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
-    } else if (al) {
-        embed_sum_launch<T, V, true>(a, s);
+        if (mode == ROWS_ALIGNED)
+            hipLaunchKernelGGL((embed_few_kernel<T, V, ROWS_ALIGNED>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
+        else if (mode == ROWS_ANY)
+            hipLaunchKernelGGL((embed_few_kernel<T, V, ROWS_ANY>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
+        else
+            hipLaunchKernelGGL((embed_few_kernel<T, V, ROWS_TINY>), grid, dim3(FEW), 0, s, ids, pad, err_flag, zero_rows, a);
+    } else if (mode == ROWS_ALIGNED) {
+        embed_sum_launch<T, V, ROWS_ALIGNED>(a, s);
+    } else if (mode == ROWS_ANY) {
+        embed_sum_launch<T, V, ROWS_ANY>(a, s);
     } else {
-        embed_sum_launch<T, V, false>(a, s);
+        embed_sum_launch<T, V, ROWS_TINY>(a, s);
     }
 }
+int rows_mode(bool al, int cols) { return al ? ROWS_ALIGNED : cols >= 8 ? ROWS_ANY : ROWS_TINY; }
 bool float_type(int dt) { return dt == BF_F32 || bf_is_half(dt); }
 
 }  // namespace
@@ -592,19 +600,20 @@ extern "C" int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int
     const unsigned vpr = (unsigned)((cols + V - 1) / V);
     const unsigned long long nvec = (unsigned long long)n * vpr;
     BF_REQUIRE(nvec <= 0x7FFFF000ull, BF_EINVAL, "%s: n=%d x cols=%d is too large", name, n, cols);
-    const bool al = cols % V == 0 && bf_aligned16(table) && bf_aligned16(out);
+    const int mode = rows_mode(cols % V == 0 && bf_aligned16(table) && bf_aligned16(out), cols);
     hipStream_t s = (hipStream_t)stream;
     // vectors a lane: many for a long batch (131 072 x 1 024 bf16: 75.9 us with four, 91.8 with one), one where the launch's
     // latency counts (8 192 x 768: 5.9 us, with four 6.3; 77 x 512: 3.0 and 3.8)
-    const int U = nvec >= (1u << 21) ? 4 : 1;
+    const int U = nvec >= (1u << 21) && mode != ROWS_TINY ? 4 : 1;
     const dim3 grid((unsigned)((nvec + 256 * U - 1) / (256 * U))), block(256);
 #define EMBED_FWD2(T, A, N)                                                                                                      \
     hipLaunchKernelGGL((embed_scaled_kernel<T, A, N>), grid, block, 0, s, tokens, (const T*)table, out, out_dtype, scale,        \
                        (unsigned)nvec, vpr, cols, vocab, err_flag)
 #define EMBED_FWD(T)                                                                                                             \
     do {                                                                                                                         \
-        if (al) { if (U == 4) EMBED_FWD2(T, true, 4); else EMBED_FWD2(T, true, 1); }                                             \
-        else { if (U == 4) EMBED_FWD2(T, false, 4); else EMBED_FWD2(T, false, 1); }                                              \
+        if (mode == ROWS_ALIGNED) { if (U == 4) EMBED_FWD2(T, ROWS_ALIGNED, 4); else EMBED_FWD2(T, ROWS_ALIGNED, 1); }           \
+        else if (mode == ROWS_ANY) { if (U == 4) EMBED_FWD2(T, ROWS_ANY, 4); else EMBED_FWD2(T, ROWS_ANY, 1); }                  \
+        else EMBED_FWD2(T, ROWS_TINY, 1);                                                                                        \
     } while (0)
     if (table_dtype == BF_F32) EMBED_FWD(float);
     else if (table_dtype == BF_BF16) EMBED_FWD(bf16_t);
@@ -642,7 +651,7 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
     const size_t esz = bf_dtype_size(dy_dtype);
     BF_REQUIRE((uintptr_t)dy % esz == 0 && (uintptr_t)tokens % 4 == 0, BF_EALIGN, "%s: a tensor is not aligned to its element", name);
     const int V = dy_dtype == BF_F32 ? 4 : 8;
-    const bool al = cols % V == 0 && bf_aligned16(dy) && ((size_t)ld_dy * esz) % 16 == 0 && bf_aligned16(grad);
+    const int mode = rows_mode(cols % V == 0 && bf_aligned16(dy) && ((size_t)ld_dy * esz) % 16 == 0 && bf_aligned16(grad), cols);
     SumArgs a = {};
     a.n = n; a.vocab = vocab; a.dy = dy; a.ld = ld_dy; a.cols = cols; a.scale = scale; a.accumulate = accumulate; a.grad = grad;
     a.slabs = (cols + 64 * V - 1) / (64 * V);
@@ -687,13 +696,16 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
         a.sorted = q.out; a.chunk = p.chunk; a.chunks = p.chunks; a.owners = owners; a.owner_count = q.owner_count;
         a.part = (float*)(ws + p.part);
     }
-    if (dy_dtype == BF_F32) embed_bwd_type<float, 4>(few, al, tokens, padding_idx, err_flag, a, s);
-    else if (dy_dtype == BF_BF16) embed_bwd_type<bf16_t, 8>(few, al, tokens, padding_idx, err_flag, a, s);
-    else embed_bwd_type<f16_t, 8>(few, al, tokens, padding_idx, err_flag, a, s);
+    if (dy_dtype == BF_F32) embed_bwd_type<float, 4>(few, mode, tokens, padding_idx, err_flag, a, s);
+    else if (dy_dtype == BF_BF16) embed_bwd_type<bf16_t, 8>(few, mode, tokens, padding_idx, err_flag, a, s);
+    else embed_bwd_type<f16_t, 8>(few, mode, tokens, padding_idx, err_flag, a, s);
     BF_CHECK_LAUNCH(name);
     if (!few) {
         const size_t most = (size_t)a.chunks * ((cols + 255) / 256);
-        hipLaunchKernelGGL(embed_join_kernel, dim3((unsigned)(most < 512 ? most : 512)), dim3(1024), 0, s, a);
+        const dim3 grid((unsigned)(most < 512 ? most : 512)), block(1024);
+        if (mode == ROWS_ALIGNED) hipLaunchKernelGGL(embed_join_kernel<ROWS_ALIGNED>, grid, block, 0, s, a);
+        else if (mode == ROWS_ANY) hipLaunchKernelGGL(embed_join_kernel<ROWS_ANY>, grid, block, 0, s, a);
+        else hipLaunchKernelGGL(embed_join_kernel<ROWS_TINY>, grid, block, 0, s, a);
         BF_CHECK_LAUNCH(name);
     }
     return BF_OK;

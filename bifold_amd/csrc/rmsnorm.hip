@@ -36,15 +36,15 @@ struct RmsBwd {
     int rows, cols, gpr, nblk;
 };
 
-template <int V, bool AL> __device__ __forceinline__ void load_as(const void* p, int dtype, size_t off, int n, float (&o)[V]) {
-    if (dtype == BF_F32) vec_load_n<float, V, AL>((const float*)p + off, n, o);
-    else if (dtype == BF_BF16) vec_load_n<bf16_t, V, AL>((const bf16_t*)p + off, n, o);
-    else vec_load_n<f16_t, V, AL>((const f16_t*)p + off, n, o);
+template <int V, int A> __device__ __forceinline__ void load_as(const void* p, int dtype, size_t off, int n, float (&o)[V]) {
+    if (dtype == BF_F32) vec_load_n<float, V, A>((const float*)p + off, n, o);
+    else if (dtype == BF_BF16) vec_load_n<bf16_t, V, A>((const bf16_t*)p + off, n, o);
+    else vec_load_n<f16_t, V, A>((const f16_t*)p + off, n, o);
 }
-template <int V, bool AL> __device__ __forceinline__ void store_as(void* p, int dtype, size_t off, int n, const float (&v)[V]) {
-    if (dtype == BF_F32) vec_store_n<float, V, AL>((float*)p + off, n, v);
-    else if (dtype == BF_BF16) vec_store_n<bf16_t, V, AL>((bf16_t*)p + off, n, v);
-    else vec_store_n<f16_t, V, AL>((f16_t*)p + off, n, v);
+template <int V, int A> __device__ __forceinline__ void store_as(void* p, int dtype, size_t off, int n, const float (&v)[V]) {
+    if (dtype == BF_F32) vec_store_n<float, V, A>((float*)p + off, n, v);
+    else if (dtype == BF_BF16) vec_store_n<bf16_t, V, A>((bf16_t*)p + off, n, v);
+    else vec_store_n<f16_t, V, A>((f16_t*)p + off, n, v);
 }
 template <int V> __device__ __forceinline__ void to_e4m3(const float (&y)[V], float inv, unsigned (&w)[V / 4]) {
 #pragma unroll
@@ -92,23 +92,23 @@ template <int WPR> __device__ __forceinline__ unsigned row_max(unsigned v, unsig
     }
     return v;
 }
-template <int V, bool AL>
+template <int V, int A>
 __device__ __forceinline__ void keep8(const RmsFwd& a, int row, int c, int n, const float (&t)[V]) {
     const unsigned code = act8_code(group_max<V>(magnitude_bits<V>(t)));
     unsigned w[V / 4];
     act8_quant<V>(t, code, w);
-    bytes_store_n<V, AL>(a.q + (size_t)row * a.cols + c, n, w);
+    bytes_store_n<V, A>(a.q + (size_t)row * a.cols + c, n, w);
     if ((c & 31) == 0 && n > 0) a.code[(size_t)row * a.gpr + (c >> 5)] = (uint8_t)code;
 }
 
-template <typename TD, int V, int T, int NV, bool AL>
+template <typename TD, int V, int T, int NV, int A>
 __device__ __forceinline__ void add_row(const RmsFwd& a, int row, int slot, float (&t)[NV][V]) {
     const TD* p = (const TD*)a.delta + (size_t)row * a.ldd;
     float d[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * T + slot) * V;
-        vec_load_n<TD, V, AL>(p + c, a.cols - c, d[i]);
+        vec_load_n<TD, V, A>(p + c, a.cols - c, d[i]);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -117,7 +117,7 @@ __device__ __forceinline__ void add_row(const RmsFwd& a, int row, int slot, floa
 }
 
 // ------------------------------------------------------------------ forward, the row in registers (cols <= 64 WPR V NV)
-template <typename TX, int V, int WPR, int NV, bool AL>
+template <typename TX, int V, int WPR, int NV, int A>
 __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
     constexpr int T = 64 * WPR;
     __shared__ float red_s[4];
@@ -130,12 +130,12 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * T + slot) * V;
-        vec_load_n<TX, V, AL>(x + c, a.cols - c, t[i]);
+        vec_load_n<TX, V, A>(x + c, a.cols - c, t[i]);
     }
     if (a.delta) {                              // all chunks' loads first: a conversion between them would wait for each
-        if (a.d_dtype == BF_F32) add_row<float, V, T, NV, AL>(a, row, slot, t);
-        else if (a.d_dtype == BF_BF16) add_row<bf16_t, V, T, NV, AL>(a, row, slot, t);
-        else add_row<f16_t, V, T, NV, AL>(a, row, slot, t);
+        if (a.d_dtype == BF_F32) add_row<float, V, T, NV, A>(a, row, slot, t);
+        else if (a.d_dtype == BF_BF16) add_row<bf16_t, V, T, NV, A>(a, row, slot, t);
+        else add_row<f16_t, V, T, NV, A>(a, row, slot, t);
     }
     float s = 0.f;
 #pragma unroll
@@ -147,14 +147,14 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
-            vec_store_n<TX, V, AL>(o + c, a.cols - c, t[i]);
+            vec_store_n<TX, V, A>(o + c, a.cols - c, t[i]);
         }
     }
     if (a.q) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
-            keep8<V, AL>(a, row, c, a.cols - c, t[i]);
+            keep8<V, A>(a, row, c, a.cols - c, t[i]);
         }
     }
     const float r = 1.0f / sqrtf(row_sum<WPR>(s, red_s) / (float)a.cols + a.eps);
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
     for (int i = 0; i < NV; ++i) {
         const int c = (i * T + slot) * V;
         float g[V];
-        vec_load_n<float, V, AL>(a.gamma + c, a.cols - c, g);
+        vec_load_n<float, V, A>(a.gamma + c, a.cols - c, g);
 #pragma unroll
         for (int j = 0; j < V; ++j) t[i][j] = t[i][j] * r * g[j];
         const unsigned b = magnitude_bits<V>(t[i]);
@@ -179,19 +179,19 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
             const int c = (i * T + slot) * V;
             unsigned w[V / 4];
             to_e4m3<V>(t[i], inv, w);
-            bytes_store_n<V, AL>((uint8_t*)a.y + yo + c, a.cols - c, w);
+            bytes_store_n<V, A>((uint8_t*)a.y + yo + c, a.cols - c, w);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
-            store_as<V, AL>(a.y, a.y_dtype, yo + c, a.cols - c, t[i]);
+            store_as<V, A>(a.y, a.y_dtype, yo + c, a.cols - c, t[i]);
         }
     }
 }
 
 // ------------------------------------------------------------------ forward, any width: one workgroup walks the row
-template <typename TX>
+template <typename TX, int A>
 __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
     constexpr int V = 8;
     __shared__ float red_s[4];
@@ -200,17 +200,17 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
     const TX* x = (const TX*)a.x + (size_t)row * a.ldx;
     // t of this thread's chunk; x is read before x_out (which may be x) is written, and only by this thread
     auto chunk = [&](int c, float (&t)[V]) __attribute__((always_inline)) {
-        vec_load_n<TX, V, false>(x + c, a.cols - c, t);
+        vec_load_n<TX, V, A>(x + c, a.cols - c, t);
         if (a.delta) {
             float d[V];
-            load_as<V, false>(a.delta, a.d_dtype, (size_t)row * a.ldd + c, a.cols - c, d);
+            load_as<V, A>(a.delta, a.d_dtype, (size_t)row * a.ldd + c, a.cols - c, d);
 #pragma unroll
             for (int j = 0; j < V; ++j) t[j] += d[j];
         }
     };
     auto scaled = [&](int c, float r, float (&t)[V]) __attribute__((always_inline)) {
         float g[V];
-        vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
+        vec_load_n<float, V, A>(a.gamma + c, a.cols - c, g);
 #pragma unroll
         for (int j = 0; j < V; ++j) t[j] = t[j] * r * g[j];
     };
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
         chunk(c, t);
 #pragma unroll
         for (int j = 0; j < V; ++j) s = fmaf(t[j], t[j], s);
-        if (a.q) keep8<V, false>(a, row, c, a.cols - c, t);
+        if (a.q) keep8<V, A>(a, row, c, a.cols - c, t);
     }
     const float r = 1.0f / sqrtf(row_sum<4>(s, red_s) / (float)a.cols + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = r;
@@ -240,14 +240,14 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
     const size_t yo = (size_t)row * a.cols;
     for (int c = threadIdx.x * V; c < a.cols; c += 256 * V) {
         chunk(c, t);
-        if (a.x_out) vec_store_n<TX, V, false>((TX*)a.x_out + (size_t)row * a.ldo + c, a.cols - c, t);
+        if (a.x_out) vec_store_n<TX, V, A>((TX*)a.x_out + (size_t)row * a.ldo + c, a.cols - c, t);
         scaled(c, r, t);
         if (a.y_dtype == Y_E4M3) {
             unsigned w[V / 4];
             to_e4m3<V>(t, inv, w);
-            bytes_store_n<V, false>((uint8_t*)a.y + yo + c, a.cols - c, w);
+            bytes_store_n<V, A>((uint8_t*)a.y + yo + c, a.cols - c, w);
         } else {
-            store_as<V, false>(a.y, a.y_dtype, yo + c, a.cols - c, t);
+            store_as<V, A>(a.y, a.y_dtype, yo + c, a.cols - c, t);
         }
     }
 }
@@ -255,20 +255,23 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwd a) {
 // ------------------------------------------------------------------ backward
 struct Kept {};                                 // the stream is a checkpoint
 
-template <typename TX, int V, bool AL> struct StreamChunk {
-    Chunk<TX, V, AL> x;
+template <typename TX, int V, int A> struct StreamChunk {
+    Chunk<TX, V, A> x;
     __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) { x.load(a.x, (size_t)row * a.ldx + c, n); }
-    __device__ __forceinline__ void take(int, float (&t)[V]) const { x.take(t); }
+    __device__ __forceinline__ void take(int n, float (&t)[V]) const { x.take(t, n); }
 };
-template <int V, bool AL> struct StreamChunk<Kept, V, AL> {
-    unsigned w[V / 4], code;
+template <int V, int A> struct StreamChunk<Kept, V, A> {
+    Chunk<uint8_t, V, A> q;
+    unsigned code;
     __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) {
-        bytes_load_n<V, AL>(a.q + (size_t)row * a.cols + c, n, w);
-        code = n > 0 ? a.code[(size_t)row * a.gpr + (c >> 5)] : 1u;
+        q.load(a.q, (size_t)row * a.cols + c, n);
+        code = a.code[(size_t)row * a.gpr + (n > 0 ? c >> 5 : 0)];
     }
     __device__ __forceinline__ void take(int n, float (&t)[V]) const {
+        unsigned w[V / 4];
+        q.words(w, n);
         act8_dequant<V>(w, code, t);
-        if (!AL && n < V) {                     // a NaN group's missing columns are no part of the row
+        if (n < V) {                            // a NaN group's missing columns are no part of the row
 #pragma unroll
             for (int j = 0; j < V; ++j) t[j] = j < n ? t[j] : 0.f;
         }
@@ -279,7 +282,7 @@ template <int V, bool AL> struct StreamChunk<Kept, V, AL> {
 // registers, the workgroup writes one row of partial sums and rms_dgamma_kernel adds those in a fixed order.  A row's three
 // loads are issued together, in the types they have (template: a branch on a type at run time would convert, and so wait,
 // between them).
-template <typename TDY, typename TX, typename TD, int V, int WPR, int NV, bool AL>
+template <typename TDY, typename TX, typename TD, int V, int WPR, int NV, int A>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
     constexpr int T = 64 * WPR;
     __shared__ float red[2][4];
@@ -291,15 +294,15 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * T + slot) * V;
-        vec_load_n<float, V, AL>(a.gamma + c, a.cols - c, g[i]);
+        vec_load_n<float, V, A>(a.gamma + c, a.cols - c, g[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[i][j] = 0.f;
     }
     int turn = 0;
     for (int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x; row < a.rows; row += stride, turn ^= 1) {
-        Chunk<TDY, V, AL> dy[NV];
-        StreamChunk<TX, V, AL> x[NV];
-        Chunk<TD, V, AL> dres[NV];
+        Chunk<TDY, V, A> dy[NV];
+        StreamChunk<TX, V, A> x[NV];
+        Chunk<TD, V, A> dres[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
@@ -317,8 +320,9 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
         float b[NV][V], h[NV][V], s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            dy[i].take(b[i]);
-            x[i].take(a.cols - (i * T + slot) * V, h[i]);
+            const int n = a.cols - (i * T + slot) * V;
+            dy[i].take(b[i], n);
+            x[i].take(n, h[i]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 h[i][j] *= r;
@@ -335,11 +339,11 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
             for (int j = 0; j < V; ++j) b[i][j] = r * (b[i][j] - h[i][j] * m);
             if (a.dres) {
                 float d[V];
-                dres[i].take(d);
+                dres[i].take(d, n);
 #pragma unroll
                 for (int j = 0; j < V; ++j) b[i][j] += d[j];
             }
-            vec_store_n<TD, V, AL>((TD*)a.dx + (size_t)row * a.cols + c, n, b[i]);
+            vec_store_n<TD, V, A>((TD*)a.dx + (size_t)row * a.cols + c, n, b[i]);
         }
     }
     float* part = a.part + (size_t)blockIdx.x * a.cols;
@@ -358,26 +362,26 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
-            vec_store_n<float, V, AL>(part + c, a.cols - c, acc[i]);
+            vec_store_n<float, V, A>(part + c, a.cols - c, acc[i]);
         }
     }
 }
 
 // t of one chunk, its type chosen at run time
-template <int V>
+template <int V, int A>
 __device__ __forceinline__ void stream_load(const RmsBwd& a, int row, int c, int n, float (&t)[V]) {
     if (a.q) {
-        StreamChunk<Kept, V, false> k;
+        StreamChunk<Kept, V, A> k;
         k.load(a, row, c, n);
         k.take(n, t);
     } else {
-        load_as<V, false>(a.x, a.x_dtype, (size_t)row * a.ldx + c, n, t);
+        load_as<V, A>(a.x, a.x_dtype, (size_t)row * a.ldx + c, n, t);
     }
 }
 
 // any width and any mixture of types: dx by one workgroup per row, two walks; dgamma by columns, a thread per column and
 // chunk of rows
-template <typename TDY>
+template <typename TDY, int A>
 __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
     constexpr int V = 8;
     __shared__ float red[4];
@@ -386,9 +390,9 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
         const float r = a.rstd[row];
         auto chunk = [&](int c, float (&b)[V], float (&h)[V]) __attribute__((always_inline)) {
             float g[V];
-            vec_load_n<TDY, V, false>(dy + c, a.cols - c, b);
-            vec_load_n<float, V, false>(a.gamma + c, a.cols - c, g);
-            stream_load<V>(a, row, c, a.cols - c, h);
+            vec_load_n<TDY, V, A>(dy + c, a.cols - c, b);
+            vec_load_n<float, V, A>(a.gamma + c, a.cols - c, g);
+            stream_load<V, A>(a, row, c, a.cols - c, h);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 b[j] *= g[j];
@@ -408,11 +412,11 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwd a) {
             for (int j = 0; j < V; ++j) b[j] = r * (b[j] - h[j] * m);
             if (a.dres) {
                 float d[V];
-                load_as<V, false>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, a.cols - c, d);
+                load_as<V, A>(a.dres, a.dx_dtype, (size_t)row * a.ldr + c, a.cols - c, d);
 #pragma unroll
                 for (int j = 0; j < V; ++j) b[j] += d[j];
             }
-            store_as<V, false>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, a.cols - c, b);
+            store_as<V, A>(a.dx, a.dx_dtype, (size_t)row * a.cols + c, a.cols - c, b);
         }
         __syncthreads();                        // red is written again
     }
@@ -429,7 +433,9 @@ __global__ __launch_bounds__(256) void rms_dgamma_long_kernel(const RmsBwd a) {
             const float step = act8_step(a.code[(size_t)row * a.gpr + (c >> 5)]);
             t[0] = (float)(int8_t)a.q[(size_t)row * a.cols + c] * step;
         } else {
-            load_as<1, false>(a.x, a.x_dtype, (size_t)row * a.ldx + c, 1, t);
+            t[0] = a.x_dtype == BF_F32 ? ((const float*)a.x)[(size_t)row * a.ldx + c]
+                 : a.x_dtype == BF_BF16 ? to_f32<bf16_t>(((const bf16_t*)a.x)[(size_t)row * a.ldx + c])
+                                        : to_f32<f16_t>(((const f16_t*)a.x)[(size_t)row * a.ldx + c]);
         }
         s = fmaf(to_f32<TDY>(((const TDY*)a.dy)[(size_t)row * a.ldy + c]), t[0] * a.rstd[row], s);
     }
@@ -462,10 +468,10 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
 #define RMS_SLICE (1 << 22)                     /* rows of one forward launch; a multiple of every alignment */
 #define RMS_MOST (1 << 30)                      /* rows, columns */
 
-template <typename TX, int V, bool AL> void rms_fwd_launch(const RmsFwd& a, hipStream_t s) {
+template <typename TX, int V, int A> void rms_fwd_launch(const RmsFwd& a, hipStream_t s) {
     const dim3 wave((unsigned)((a.rows + 3) / 4)), wg((unsigned)a.rows), block(256);
     const int chunks = (a.cols + V - 1) / V;
-#define RMS_FWD(W, N) hipLaunchKernelGGL((rms_fwd_kernel<TX, V, W, N, AL>), W == 1 ? wave : wg, block, 0, s, a)
+#define RMS_FWD(W, N) hipLaunchKernelGGL((rms_fwd_kernel<TX, V, W, N, A>), W == 1 ? wave : wg, block, 0, s, a)
     if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
         if (chunks <= 64) RMS_FWD(1, 1);
         else if (chunks <= 128) RMS_FWD(1, 2);
@@ -477,17 +483,18 @@ template <typename TX, int V, bool AL> void rms_fwd_launch(const RmsFwd& a, hipS
     } else {
         if (chunks <= 64) RMS_FWD(1, 1);
         else if (chunks <= 128) RMS_FWD(1, 2);
+        else if (chunks <= 192) RMS_FWD(1, 3);  // 40 000 x 1 536: 70 us, as a workgroup per row 75; 16 384 x 2 048: 36 and 32
         else if (chunks <= 256) RMS_FWD(4, 1);
         else if (chunks <= 512) RMS_FWD(4, 2);
         else RMS_FWD(4, 4);
     }
 #undef RMS_FWD
 }
-template <typename TDY, typename TX, typename TD, int V, bool AL> void rms_bwd_launch(const RmsBwd& a, hipStream_t s) {
+template <typename TDY, typename TX, typename TD, int V, int A> void rms_bwd_launch(const RmsBwd& a, hipStream_t s) {
     const dim3 grid((unsigned)a.nblk), block(256);
     const int chunks = (a.cols + V - 1) / V;
     const size_t lds = (size_t)16 * a.cols;     // WPR == 1: at most 16 KB
-#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, TX, TD, V, W, N, AL>), grid, block, W == 1 ? lds : 0, s, a)
+#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, TX, TD, V, W, N, A>), grid, block, W == 1 ? lds : 0, s, a)
     if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
         if (chunks <= 64) RMS_BWD(1, 1);
         else if (chunks <= 128) RMS_BWD(1, 2);
@@ -508,27 +515,30 @@ template <typename TDY, typename TX, typename TD, int V, bool AL> void rms_bwd_l
 
 template <typename TX> void rms_fwd_any(const RmsFwd& a, bool al, hipStream_t s) {
     constexpr int V = sizeof(TX) == 4 ? 4 : 8;
-    if (a.cols > RMS_LONG) hipLaunchKernelGGL((rms_fwd_long_kernel<TX>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
-    else if (al) rms_fwd_launch<TX, V, true>(a, s);
-    else rms_fwd_launch<TX, V, false>(a, s);
+    if (a.cols < 8) hipLaunchKernelGGL((rms_fwd_long_kernel<TX, ROWS_TINY>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    else if (a.cols > RMS_LONG) hipLaunchKernelGGL((rms_fwd_long_kernel<TX, ROWS_ANY>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    else if (al) rms_fwd_launch<TX, V, ROWS_ALIGNED>(a, s);
+    else rms_fwd_launch<TX, V, ROWS_ANY>(a, s);
 }
 template <typename TDY, typename TX, typename TD> void rms_bwd_types(const RmsBwd& a, bool al, hipStream_t s) {
     constexpr int V = sizeof(TDY) == 4 ? 4 : 8;
-    if (al) rms_bwd_launch<TDY, TX, TD, V, true>(a, s);
-    else rms_bwd_launch<TDY, TX, TD, V, false>(a, s);
+    if (al) rms_bwd_launch<TDY, TX, TD, V, ROWS_ALIGNED>(a, s);
+    else rms_bwd_launch<TDY, TX, TD, V, ROWS_ANY>(a, s);
 }
-// dy, x and dx of one 16-bit type or fp32, with dy fp32 only beside fp32: what training steps have.  Wider rows and other
-// mixtures take the kernels that walk.
+// dy, x and dx of one 16-bit type or fp32, with dy fp32 only beside fp32: what training steps have.  Wider rows, rows under 8
+// columns and other mixtures take the kernels that walk.
 template <typename TDY> constexpr int dtype_of() { return sizeof(TDY) == 4 ? BF_F32 : __is_same(TDY, bf16_t) ? BF_BF16 : BF_F16; }
 bool rms_bwd_walks(int dy_dtype, int x_dtype, bool kept, int dx_dtype, int cols) {
     const bool x_ok = kept || x_dtype == BF_F32 || x_dtype == dy_dtype, d_ok = dx_dtype == BF_F32 || dx_dtype == dy_dtype;
-    return cols > RMS_LONG || !x_ok || !d_ok;
+    return cols < 8 || cols > RMS_LONG || !x_ok || !d_ok;
 }
 template <typename TDY> void rms_bwd_any(const RmsBwd& a, bool al, hipStream_t s) {
     constexpr int dt = dtype_of<TDY>();
     if (rms_bwd_walks(dt, a.x_dtype, a.q != nullptr, a.dx_dtype, a.cols)) {
         hipLaunchKernelGGL((rms_dgamma_long_kernel<TDY>), dim3((unsigned)((a.cols + 255) / 256), (unsigned)a.nblk), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((rms_bwd_long_kernel<TDY>), dim3((unsigned)(a.rows < RMS_SLICE ? a.rows : RMS_SLICE)), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)(a.rows < RMS_SLICE ? a.rows : RMS_SLICE));
+        if (a.cols < 8) hipLaunchKernelGGL((rms_bwd_long_kernel<TDY, ROWS_TINY>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((rms_bwd_long_kernel<TDY, ROWS_ANY>), grid, dim3(256), 0, s, a);
     } else if (a.dx_dtype == dt) {
         if (a.q) rms_bwd_types<TDY, Kept, TDY>(a, al, s);
         else if (a.x_dtype == dt) rms_bwd_types<TDY, TDY, TDY>(a, al, s);
@@ -613,10 +623,11 @@ extern "C" int bf_rmsnorm_fwd_fp8(const void* x, int64_t ldx, int x_dtype, const
 extern "C" int bf_rmsnorm_bwd_parts(int rows, int cols) {
     if (rows <= 0 || cols <= 0) return 0;
     if (cols > RMS_LONG) return rows < 64 ? rows : 64;
-    // a row per wave: up to 1 024 workgroups of four rows side by side; a row per workgroup: half as many partial rows, each
-    // up to 32 KB
+    // As many workgroups as stay resident side by side: their registers grow with the row (9 000 x 4 096: 48 us with 1 024,
+    // 55 with 512 or 2 048; 4 096 x 8 192: 44 with 512, 55 with 1 024; 40 000 x 1 536: 86 with 1 280, 93 with 1 024).
     if (cols <= 1024) return (rows + 3) / 4 < 1024 ? (rows + 3) / 4 : 1024;
-    return rows < 512 ? rows : 512;
+    const int most = cols <= 2048 ? 1280 : cols <= 4096 ? 1024 : 512;
+    return rows < most ? rows : most;
 }
 
 extern "C" int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const void* x, int64_t ldx, int x_dtype, const void* q,
