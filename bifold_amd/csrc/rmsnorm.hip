@@ -8,8 +8,8 @@
 //
 // HBM bounds both: each tensor is read once and written once, the row stays in registers between the sum and the output.  A
 // lane holds V consecutive elements per chunk: 4 of an fp32 stream, 8 of a 16-bit one (16 bytes either way).  Rows up to
-// 1 024 columns belong to one wave (reductions without LDS or barriers, four rows per workgroup); up to 8 192 to one
-// workgroup; longer ones are walked two or three times.  Measured: 50 432 x 768, fp32 stream + fp16 branch to e4m3, sum written:
+// 1 024 columns belong to one wave (reductions without LDS or barriers, four rows per workgroup); up to 16 384 to one
+// workgroup (of four waves, over 8 192 of sixteen); longer ones are walked two or three times.  Measured: 50 432 x 768, fp32 stream + fp16 branch to e4m3, sum written:
 // 79 us, 5.4 TB/s; 36 928 x 1 024 to fp16 with the checkpoint 85 us, 5.8 TB/s, and its backward from the checkpoint 62 + 5 us,
 // 4.4 TB/s (a copy of 2 GiB reaches 4.9, one of 256 MiB 5.5); next-row loads issued before a row's arithmetic changed nothing.
 #include "act8.h"
@@ -120,10 +120,10 @@ __device__ __forceinline__ void add_row(const RmsFwd& a, int row, int slot, floa
 
 // ------------------------------------------------------------------ forward, the row in registers (cols <= 64 WPR V NV)
 template <typename TX, int V, int WPR, int NV, int A>
-__global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwd a) {
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void rms_fwd_kernel(const RmsFwd a) {
     constexpr int T = 64 * WPR;
-    __shared__ float red_s[4];
-    __shared__ unsigned red_m[4];
+    __shared__ float red_s[WPR];
+    __shared__ unsigned red_m[WPR];
     const int row = WPR == 1 ? blockIdx.x * 4 + wave_id() : blockIdx.x;
     if (row >= a.rows) return;
     const int slot = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -285,9 +285,9 @@ template <int V, int A> struct StreamChunk<Kept, V, A> {
 // loads are issued together, in the types they have (template: a branch on a type at run time would convert, and so wait,
 // between them).
 template <typename TDY, typename TX, typename TD, int V, int WPR, int NV, int A>
-__global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwd a) {
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void rms_bwd_kernel(const RmsBwd a) {
     constexpr int T = 64 * WPR;
-    __shared__ float red[2][4];
+    __shared__ float red[2][WPR];
     extern __shared__ float fold[];             // WPR == 1: [4][cols]
     const int wave = wave_id();
     const int slot = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -466,29 +466,31 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
 }
 
 // ------------------------------------------------------------------ dispatch
-#define RMS_LONG 8192                           /* widest row kept in the registers of one workgroup */
+#define RMS_LONG 16384                          /* widest row kept in the registers of one workgroup */
 #define RMS_SLICE (1 << 22)                     /* rows of one forward launch; a multiple of every alignment */
 #define RMS_MOST (1 << 30)                      /* rows, columns */
 
 template <typename TX, int V, int A> void rms_fwd_launch(const RmsFwd& a, hipStream_t s) {
     const dim3 wave((unsigned)((a.rows + 3) / 4)), wg((unsigned)a.rows), block(256);
     const int chunks = (a.cols + V - 1) / V;
-#define RMS_FWD(W, N) hipLaunchKernelGGL((rms_fwd_kernel<TX, V, W, N, A>), W == 1 ? wave : wg, block, 0, s, a)
-    if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
+#define RMS_FWD(W, N) hipLaunchKernelGGL((rms_fwd_kernel<TX, V, W, N, A>), W == 1 ? wave : wg, W == 16 ? dim3(1024) : block, 0, s, a)
+    if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to four, 16 384 to sixteen
         if (chunks <= 64) RMS_FWD(1, 1);
         else if (chunks <= 128) RMS_FWD(1, 2);
         else if (chunks <= 192) RMS_FWD(1, 3);
         else if (chunks <= 256) RMS_FWD(1, 4);
         else if (chunks <= 512) RMS_FWD(4, 2);
         else if (chunks <= 1024) RMS_FWD(4, 4);
-        else RMS_FWD(4, 8);
+        else if (chunks <= 2048) RMS_FWD(4, 8);
+        else RMS_FWD(16, 4);
     } else {
         if (chunks <= 64) RMS_FWD(1, 1);
         else if (chunks <= 128) RMS_FWD(1, 2);
         else if (chunks <= 192) RMS_FWD(1, 3);  // 40 000 x 1 536: 70 us, as a workgroup per row 75; 16 384 x 2 048: 36 and 32
         else if (chunks <= 256) RMS_FWD(4, 1);
         else if (chunks <= 512) RMS_FWD(4, 2);
-        else RMS_FWD(4, 4);
+        else if (chunks <= 1024) RMS_FWD(4, 4);
+        else RMS_FWD(16, 2);
     }
 #undef RMS_FWD
 }
@@ -496,21 +498,23 @@ template <typename TDY, typename TX, typename TD, int V, int A> void rms_bwd_lau
     const dim3 grid((unsigned)a.nblk), block(256);
     const int chunks = (a.cols + V - 1) / V;
     const size_t lds = (size_t)16 * a.cols;     // WPR == 1: at most 16 KB
-#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, TX, TD, V, W, N, A>), grid, block, W == 1 ? lds : 0, s, a)
-    if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to a workgroup
+#define RMS_BWD(W, N) hipLaunchKernelGGL((rms_bwd_kernel<TDY, TX, TD, V, W, N, A>), grid, W == 16 ? dim3(1024) : block, W == 1 ? lds : 0, s, a)
+    if constexpr (V == 4) {                      // 1 024 columns to a wave, 8 192 to four, 16 384 to sixteen
         if (chunks <= 64) RMS_BWD(1, 1);
         else if (chunks <= 128) RMS_BWD(1, 2);
         else if (chunks <= 192) RMS_BWD(1, 3);
         else if (chunks <= 256) RMS_BWD(1, 4);
         else if (chunks <= 512) RMS_BWD(4, 2);
         else if (chunks <= 1024) RMS_BWD(4, 4);
-        else RMS_BWD(4, 8);
+        else if (chunks <= 2048) RMS_BWD(4, 8);
+        else RMS_BWD(16, 4);
     } else {
         if (chunks <= 64) RMS_BWD(1, 1);
         else if (chunks <= 128) RMS_BWD(1, 2);
         else if (chunks <= 256) RMS_BWD(4, 1);
         else if (chunks <= 512) RMS_BWD(4, 2);
-        else RMS_BWD(4, 4);
+        else if (chunks <= 1024) RMS_BWD(4, 4);
+        else RMS_BWD(16, 2);
     }
 #undef RMS_BWD
 }
@@ -628,7 +632,7 @@ extern "C" int bf_rmsnorm_bwd_parts(int rows, int cols) {
     // As many workgroups as stay resident side by side: their registers grow with the row (9 000 x 4 096: 48 us with 1 024,
     // 55 with 512 or 2 048; 4 096 x 8 192: 44 with 512, 55 with 1 024; 40 000 x 1 536: 86 with 1 280, 93 with 1 024).
     if (cols <= 1024) return (rows + 3) / 4 < 1024 ? (rows + 3) / 4 : 1024;
-    const int most = cols <= 2048 ? 1280 : cols <= 4096 ? 1024 : 512;
+    const int most = cols <= 2048 ? 1280 : cols <= 4096 ? 1024 : cols <= 8192 ? 512 : 256;
     return rows < most ? rows : most;
 }
 

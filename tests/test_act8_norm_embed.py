@@ -75,8 +75,8 @@ def test_rmsnorm_refusals(L):
     refused(L, bwd(dres=2 * PTR, ldr=72), -1, "rows coincide")
     refused(L, bwd(rstd=PTR + 1), -2, "aligned")
     assert [lib.bf_rmsnorm_bwd_parts(r, c) for r, c in ((0, 64), (1, 64), (5, 64), (10 ** 6, 64), (7, 4096), (9000, 2048),
-                                                         (9000, 4096), (9000, 8192), (9000, 9000))] \
-        == [0, 1, 2, 1024, 7, 1280, 1024, 512, 64]
+                                                         (9000, 4096), (9000, 8192), (9000, 9000), (9000, 20000))] \
+        == [0, 1, 2, 1024, 7, 1280, 1024, 512, 256, 64]
 
 
 def test_embedding_refusals(L):

@@ -216,7 +216,7 @@ def test_act8_gelu_non_finite_and_far(ops, L, gpu):
 
 # ------------------------------------------------------------------ RMS norm
 NORMS = [(1, 1), (1, 64), (3, 7), (7, 255), (130, 256), (9, 257), (70, 768), (33, 1000), (66, 1024), (5, 1025), (17, 1155), (6, 2048),
-         (3, 4096), (2, 4100), (4, 8192), (3, 8200), (2, 20001)]
+         (3, 4096), (2, 4100), (4, 8192), (3, 8200), (2, 12001), (3, 16384), (2, 20001)]
 PAIRS = [(torch.float32, None), (torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.float32, torch.float16),
          (torch.bfloat16, None), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.bfloat16, torch.float32)]
 
@@ -534,6 +534,25 @@ def test_very_many_rows(ops, gpu):
         assert torch.isfinite(dg).all()
 
 
+def test_batched_rows(ops, gpu):
+    """[batch, tokens, cols] tensors are rows of cols: the same bits as their two-dimensional views."""
+    g = torch.Generator().manual_seed(8)
+    x, dy = (torch.randn(3, 5, 200, generator=g).to(gpu) for _ in range(2))
+    delta, gamma = torch.randn(3, 5, 200, generator=g).half().to(gpu), torch.rand(200, generator=g).to(gpu)
+    y, rstd, kept = ops.rmsnorm_fwd(x, gamma, torch.float16, delta=delta, x_out=torch.empty_like(x), save_stats=True, checkpoint=True)
+    y2, rstd2, kept2 = ops.rmsnorm_fwd(x.view(15, 200), gamma, torch.float16, delta=delta.view(15, 200),
+                                       x_out=torch.empty(15, 200, device=gpu), save_stats=True, checkpoint=True)
+    assert y.shape == x.shape and torch.equal(y.view(15, 200), y2) and torch.equal(rstd, rstd2)
+    assert torch.equal(kept[0].view(15, 200), kept2[0]) and torch.equal(kept[1].view(15, 7), kept2[1])
+    dg, dg2 = torch.empty(200, device=gpu), torch.empty(200, device=gpu)
+    dx = ops.rmsnorm_bwd(dy, kept, gamma, rstd, dg)
+    assert torch.equal(dx.view(15, 200), ops.rmsnorm_bwd(dy.view(15, 200), kept2, gamma, rstd, dg2)) and torch.equal(dg, dg2)
+    ids = torch.randint(0, 40, (3, 5), generator=g).int().to(gpu)
+    assert torch.equal(ops.embed_scaled_bwd(dy, ids, 40, 2.0), ops.embed_scaled_bwd(dy.view(15, 200), ids.view(15), 40, 2.0))
+    one = ops.act8_pack(x[0, 0])                               # a single row
+    assert torch.equal(ops.act8_unpack(one, torch.float32), ops.act8_unpack(ops.act8_pack(x), torch.float32)[0, 0])
+
+
 def test_branch_that_is_the_stream(ops, gpu):
     for cols in (64, 1500, 9000):
         x = torch.randn(6, cols, device=gpu)
@@ -560,7 +579,7 @@ def fresh(n, vocab, cols, seed):
                 gamma=(1 + 0.1 * torch.randn(cols, generator=g)).cuda(), delta=torch.randn(n, cols, generator=g).half().cuda())
 
 
-@pytest.mark.parametrize("n", [300, 3000])
+@pytest.mark.parametrize("n", [300, 1500, 3000])
 def test_captured_step_replays_like_the_eager_one(ops, L, gpu, n):
     s = fresh(n, 700, 200, 1)
     step(ops, L, s)

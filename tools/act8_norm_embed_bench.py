@@ -37,7 +37,7 @@ for rows, cols, dt in ((36928, 4096, torch.float16), (20000, 1155, torch.bfloat1
     line("act8_gelu_fwd (tanh)", us(lambda: ops.act8_gelu_fwd(x, L.ACT_TANH_GELU)), m * (2 * e + 1.03))
     line("act8_gelu_bwd (tanh)", us(lambda: ops.act8_gelu_bwd(x, kept, L.ACT_TANH_GELU)), m * (2 * e + 1.03))
 for rows, cols in ((1, 4096), (300, 4096), (2100, 1100), (20000, 1155), (36928, 1024), (40000, 1536), (16384, 2048), (9000, 4096),
-                   (4096, 8192), (2000, 20000)):
+                   (4096, 8192), (3000, 12288), (2000, 16384), (2000, 20000)):
     x = torch.randn(rows, cols, device="cuda").half()
     g, dg, delta = torch.ones(cols, device="cuda"), torch.empty(cols, device="cuda"), torch.randn_like(x)
     _, r, kept = ops.rmsnorm_fwd(x, g, torch.float16, save_stats=True, checkpoint=True)
