@@ -38,14 +38,20 @@ template <int W> __device__ __forceinline__ void shift_down(unsigned (&w)[W], in
 template <typename T, int V, int A> struct Chunk {
     static constexpr int W = V * (int)sizeof(T) / 4;
     unsigned w[W];
-    __device__ __forceinline__ void load(const void* base, size_t off, int n) {
+    // ONCE: the kernel reads these words once and aligned rows take non-temporal loads, which leave the caches' lines to
+    // others.  36 928 x 1 024 fp16 behind a producer that wrote the operands last / behind 1 GiB of other writes: RMS norm
+    // forward with an add 47 / 58 us (ordinary loads 49 / 74), backward from the checkpoint 53 / 60 (54 / 94), GELU with its
+    // checkpoint 32 / 35 (38 / 47).  Rows of ROWS_ANY share cache lines between lanes and lose by it where the operands were
+    // written last (20 000 x 1 155 bf16 forward 41 instead of 36 us), so they keep ordinary loads.  Non-temporal stores gain
+    // nothing and cost the unpacking of 73 728 x 768 fp32 84 us instead of 46.
+    template <bool ONCE = false> __device__ __forceinline__ void load(const void* base, size_t off, int n) {
         const T* p = (const T*)base + off;
         if constexpr (A == ROWS_ANY) {
-            __builtin_memcpy(w, p + min(0, n - V), sizeof(w));
+            get<false, sizeof(T)>(p + min(0, n - V));
         } else if constexpr (A == ROWS_ALIGNED) {
 #pragma unroll
             for (int k = 0; k < W; ++k) w[k] = 0;
-            if (n >= V) __builtin_memcpy(w, __builtin_assume_aligned(p, sizeof(w) < 16 ? sizeof(w) : 16), sizeof(w));
+            if (n >= V) get<ONCE, sizeof(w) < 16 ? sizeof(w) : 16>(p);
         } else {
             T t[V];
 #pragma unroll
@@ -54,6 +60,16 @@ template <typename T, int V, int A> struct Chunk {
                 if (j < n) t[j] = p[j];
             }
             __builtin_memcpy(w, t, sizeof(w));
+        }
+    }
+    template <bool ONCE, int ALIGN> __device__ __forceinline__ void get(const T* p) {
+        typedef unsigned piece __attribute__((ext_vector_type(W > 4 ? 4 : W), aligned(ALIGN)));
+#pragma unroll
+        for (int k = 0; k < W; k += 4) {
+            piece q;
+            if constexpr (ONCE) q = __builtin_nontemporal_load((const piece*)p + k / 4);
+            else q = *((const piece*)p + k / 4);
+            __builtin_memcpy(w + k, &q, sizeof(w) < 16 ? sizeof(w) : 16);
         }
     }
     // the words, zeros behind the row's end
@@ -78,9 +94,9 @@ template <typename T, int V, int A> struct Chunk {
         for (int k = 0; k < W; ++k) asm volatile("" : "+v"(w[k]));
     }
 };
-template <typename T, int V, int A> __device__ __forceinline__ void vec_load_n(const T* p, int n, float (&o)[V]) {
+template <typename T, int V, int A, bool ONCE = false> __device__ __forceinline__ void vec_load_n(const T* p, int n, float (&o)[V]) {
     Chunk<T, V, A> c;
-    c.load(p, 0, n);
+    c.template load<ONCE>(p, 0, n);
     c.take(o, n);
 }
 template <typename T, int V, int A> __device__ __forceinline__ void vec_store_n(T* p, int n, const float (&v)[V]) {

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
     float f[V];
     unsigned w[V / 4], code;
     if constexpr (MODE == A8_PACK || MODE == A8_FWD) {
-        vec_load_n<T, V, A>(x, n, f);
+        vec_load_n<T, V, A, true>(x, n, f);
         code = act8_code(group_max<V>(magnitude_bits<V>(f)));
         act8_quant<V>(f, code, w);
         bytes_store_n<V, A>(a.q + off_q, put, w);
@@ -98,9 +98,9 @@ __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
     } else {
         Chunk<T, V, A> dy;
         Chunk<uint8_t, V, A> q;
-        q.load(a.q, off_q, n);
+        q.template load<true>(a.q, off_q, n);
         code = n > 0 ? a.code[off_c] : 1u;
-        if constexpr (MODE == A8_BWD) dy.load(x, 0, n);
+        if constexpr (MODE == A8_BWD) dy.template load<true>(x, 0, n);
         q.words(w, n);
         act8_dequant<V>(w, code, f);
         if constexpr (MODE == A8_BWD) {
@@ -116,8 +116,8 @@ __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
 template <typename T, int MODE, int ACT>
 void act8_launch(const A8Args& a, bool dense, hipStream_t s) {
     if (dense) {
-        // fp32 writers of q take 4 elements a lane (whole lines per load instruction): 73 728 x 768 packed in 56.4 us, with 8
-        // in 61.5; the read-back takes 8 (44.7 us, with 4 in 47.8)
+        // fp32 writers of q take 4 elements a lane (whole lines per load instruction): 50 432 x 768 packed in 36 us,
+        // with 8 in 38, GELU with its checkpoint 57 and 61; the read-back takes 8 (73 728 x 768 in 45 us, with 4 in 48)
         constexpr int V = sizeof(T) == 4 && MODE != A8_UNPACK ? 4 : 8;
         A8Args b = a;
         b.nvec = a.nvec * (8 / V);

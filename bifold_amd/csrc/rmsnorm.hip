@@ -110,7 +110,7 @@ __device__ __forceinline__ void add_row(const RmsFwd& a, int row, int slot, floa
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * T + slot) * V;
-        vec_load_n<TD, V, A>(p + c, a.cols - c, d[i]);
+        vec_load_n<TD, V, A, true>(p + c, a.cols - c, d[i]);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void rms_fwd_kernel(const R
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * T + slot) * V;
-        vec_load_n<TX, V, A>(x + c, a.cols - c, t[i]);
+        vec_load_n<TX, V, A, true>(x + c, a.cols - c, t[i]);
     }
     if (a.delta) {                              // all chunks' loads first: a conversion between them would wait for each
         if (a.d_dtype == BF_F32) add_row<float, V, T, NV, A>(a, row, slot, t);
@@ -259,14 +259,14 @@ struct Kept {};                                 // the stream is a checkpoint
 
 template <typename TX, int V, int A> struct StreamChunk {
     Chunk<TX, V, A> x;
-    __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) { x.load(a.x, (size_t)row * a.ldx + c, n); }
+    __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) { x.template load<true>(a.x, (size_t)row * a.ldx + c, n); }
     __device__ __forceinline__ void take(int n, float (&t)[V]) const { x.take(t, n); }
 };
 template <int V, int A> struct StreamChunk<Kept, V, A> {
     Chunk<uint8_t, V, A> q;
     unsigned code;
     __device__ __forceinline__ void load(const RmsBwd& a, int row, int c, int n) {
-        q.load(a.q, (size_t)row * a.cols + c, n);
+        q.template load<true>(a.q, (size_t)row * a.cols + c, n);
         code = a.code[(size_t)row * a.gpr + (n > 0 ? c >> 5 : 0)];
     }
     __device__ __forceinline__ void take(int n, float (&t)[V]) const {
@@ -308,14 +308,14 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void rms_bwd_kernel(const R
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * T + slot) * V;
-            dy[i].load(a.dy, (size_t)row * a.ldy + c, a.cols - c);
+            dy[i].template load<true>(a.dy, (size_t)row * a.ldy + c, a.cols - c);
             x[i].load(a, row, c, a.cols - c);
         }
         if (a.dres) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * T + slot) * V;
-                dres[i].load(a.dres, (size_t)row * a.ldr + c, a.cols - c);
+                dres[i].template load<true>(a.dres, (size_t)row * a.ldr + c, a.cols - c);
             }
         }
         const float r = a.rstd[row];
@@ -486,7 +486,7 @@ template <typename TX, int V, int A> void rms_fwd_launch(const RmsFwd& a, hipStr
     } else {
         if (chunks <= 64) RMS_FWD(1, 1);
         else if (chunks <= 128) RMS_FWD(1, 2);
-        else if (chunks <= 192) RMS_FWD(1, 3);  // 40 000 x 1 536: 70 us, as a workgroup per row 75; 16 384 x 2 048: 36 and 32
+        else if (chunks <= 192) RMS_FWD(1, 3);  // 40 000 x 1 536 with an add: 77 us, as a workgroup per row 85; 16 384 x 2 048: 36 and 32
         else if (chunks <= 256) RMS_FWD(4, 1);
         else if (chunks <= 512) RMS_FWD(4, 2);
         else if (chunks <= 1024) RMS_FWD(4, 4);
@@ -629,10 +629,16 @@ extern "C" int bf_rmsnorm_fwd_fp8(const void* x, int64_t ldx, int x_dtype, const
 extern "C" int bf_rmsnorm_bwd_parts(int rows, int cols) {
     if (rows <= 0 || cols <= 0) return 0;
     if (cols > RMS_LONG) return rows < 64 ? rows : 64;
-    // As many workgroups as stay resident side by side: their registers grow with the row (9 000 x 4 096: 48 us with 1 024,
-    // 55 with 512 or 2 048; 4 096 x 8 192: 44 with 512, 55 with 1 024; 40 000 x 1 536: 86 with 1 280, 93 with 1 024).
-    if (cols <= 1024) return (rows + 3) / 4 < 1024 ? (rows + 3) / 4 : 1024;
-    const int most = cols <= 2048 ? 1280 : cols <= 4096 ? 1024 : cols <= 8192 ? 512 : 256;
+    // As many workgroups as stay resident side by side: their registers grow with the row.  From the checkpoint with dres,
+    // operands just written: 36 928 x 1 024 fp32 85 us with 768, 106 with 1 024, 95 with 512 (fp16 51, 52, 51); 50 432 x 768
+    // fp16 51 with 768, 55 with 1 024; 60 000 x 512 fp16 45 and 43; 30 000 x 1 536 fp16 67 with 1 280, 72 with 1 024, 79 with
+    // 768; 9 000 x 4 096 fp32 86 with 768, 106 with 1 024, 101 with 512 (fp16 49, 53, 51); 4 096 x 8 192 fp32 98 with 512, 110
+    // with 768.
+    if (cols <= 1024) {                          // a wave per row
+        const int most = cols <= 512 ? 1024 : 768, want = rows / 4 + (rows % 4 != 0);
+        return want < most ? want : most;
+    }
+    const int most = cols <= 2048 ? 1280 : cols <= 4096 ? 768 : cols <= 8192 ? 512 : 256;
     return rows < most ? rows : most;
 }
 

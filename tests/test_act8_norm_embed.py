@@ -74,9 +74,10 @@ def test_rmsnorm_refusals(L):
     refused(L, bwd(dx=PTR, dxd=L.F32), -1, "rows coincide")
     refused(L, bwd(dres=2 * PTR, ldr=72), -1, "rows coincide")
     refused(L, bwd(rstd=PTR + 1), -2, "aligned")
-    assert [lib.bf_rmsnorm_bwd_parts(r, c) for r, c in ((0, 64), (1, 64), (5, 64), (10 ** 6, 64), (7, 4096), (9000, 2048),
-                                                         (9000, 4096), (9000, 8192), (9000, 9000), (9000, 20000))] \
-        == [0, 1, 2, 1024, 7, 1280, 1024, 512, 256, 64]
+    for rows, cols in ((0, 64), (1, 64), (5, 64), (10 ** 6, 64), (2 ** 31 - 129, 64), (7, 4096), (9000, 1024), (9000, 2048),
+                       (9000, 4096), (9000, 8192), (9000, 9000), (9000, 20000), (3, 20000)):
+        parts = lib.bf_rmsnorm_bwd_parts(rows, cols)
+        assert (parts == 0) if rows == 0 else (1 <= parts <= min(rows, 1280)), (rows, cols, parts)
 
 
 def test_embedding_refusals(L):
