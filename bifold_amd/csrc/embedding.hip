@@ -285,9 +285,10 @@ __device__ __forceinline__ void grad_write(const SumArgs& a, int key, int c, con
 // embed_join_kernel), its sums over the chunks it reaches into go to part[.][0].
 // The wave's number is taken as a scalar, so what follows from it (addresses, branches) is scalar; all loads of a batch have
 // arrived before its sums begin: with a wait per row, stores of finished runs between them were waited for too.
-// 131 072 x 1 024 bf16, vocabulary 65 536, 61 000 rows alive: 93 us for some 400 MB, 4.3 TB/s; 8 192 x 768 fp16, 32 000:
-// 18.5 us for 111 MB, 6.0 TB/s.
-template <typename T, int V, int A>
+// 131 072 x 1 024 bf16, vocabulary 65 536, 61 000 rows alive: 80 us for some 400 MB, 5.0 TB/s; 8 192 x 768 fp16, 32 000:
+// 19 us for 111 MB, 5.8 TB/s.  ONCE: dy past the caches (the whole gradient of the first, dy behind other writes:
+// 149 us, with ordinary loads 175; dy just written: 138 either way).
+template <typename T, int V, int A, bool ONCE>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
     const int lane = threadIdx.x & 63;
     if (blockIdx.x >= a.sum_blocks) {           // a wave per eight rows of the table
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
         for (int u = 0; u < 8; ++u) {
             const int at = min(i + u, stop - 1);
             const int row = at < here ? __builtin_amdgcn_readlane(il, at) : __builtin_amdgcn_readlane(in, at - here);
-            f[u].load(a.dy, (size_t)row * a.ld + c, nc);
+            f[u].template load<ONCE>(a.dy, (size_t)row * a.ld + c, nc);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) f[u].arrived();
@@ -558,7 +559,12 @@ template <typename T, int V, int A>
 void embed_sum_launch(SumArgs a, hipStream_t s) {
     a.sum_blocks = (unsigned)(((size_t)a.chunks * a.slabs + 3) / 4);
     const unsigned zeros = a.present ? (unsigned)(((size_t)a.vocab + 31) / 32) : 0u;
-    hipLaunchKernelGGL((embed_sum_kernel<T, V, A>), dim3(a.sum_blocks + zeros), dim3(256), 0, s, a);
+    const dim3 grid(a.sum_blocks + zeros);
+    // a dy larger than the L2 caches is read past them (12 MB read again and again: 22 us so, 19 through the caches)
+    if (A == ROWS_ALIGNED && (size_t)a.n * a.cols * sizeof(T) >= (size_t)32 << 20)
+        hipLaunchKernelGGL((embed_sum_kernel<T, V, A, A == ROWS_ALIGNED>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((embed_sum_kernel<T, V, A, false>), grid, dim3(256), 0, s, a);
 }
 template <typename T, int V>
 void embed_bwd_type(bool few, int mode, const int32_t* ids, int pad, int* err_flag, const SumArgs& a, hipStream_t s) {
