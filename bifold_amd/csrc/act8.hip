@@ -155,9 +155,9 @@ int act8_run(const char* name, const void* x, int64_t ldx, void* y, int64_t ldy,
     a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy; a.q = (uint8_t*)q; a.code = (uint8_t*)code;
     a.cols = cols; a.gpr = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
     a.vpr = (unsigned)a.gpr * 4;
-    const unsigned long long nvec = (unsigned long long)rows * a.vpr;
-    BF_REQUIRE(nvec <= 0x7FFFF000ull, BF_EINVAL, "%s: rows=%lld x cols=%d is over 2^34 elements", name, (long long)rows, cols);
-    a.nvec = (unsigned)nvec;
+    BF_REQUIRE(rows <= (int64_t)(0x7FFFF000u / a.vpr), BF_EINVAL, "%s: rows=%lld x cols=%d is over 2^34 elements", name,
+               (long long)rows, cols);
+    a.nvec = (unsigned)rows * a.vpr;
     const bool dense = cols % ACT8_GROUP == 0 && (!HAS_X || (ldx == cols && bf_aligned16(x))) &&
                        (!HAS_Y || (ldy == cols && bf_aligned16(y))) && ((uintptr_t)q & 7u) == 0;
     hipStream_t s = (hipStream_t)stream;

@@ -467,7 +467,8 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
 
 // ------------------------------------------------------------------ dispatch
 #define RMS_LONG 16384                          /* widest row kept in the registers of one workgroup */
-#define RMS_SLICE (1 << 22)                     /* rows of one forward launch; a multiple of every alignment */
+#define RMS_SLICE (1 << 21)                     /* rows of one forward launch; a multiple of every alignment */
+static_assert((unsigned long long)RMS_SLICE * 1024 < 1ull << 32, "a grid counts threads in 32 bits");
 #define RMS_MOST (1 << 30)                      /* rows, columns */
 
 template <typename TX, int V, int A> void rms_fwd_launch(const RmsFwd& a, hipStream_t s) {

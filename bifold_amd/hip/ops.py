@@ -1228,6 +1228,8 @@ def _rms_args(x, gamma, delta, x_out, write_x):
                 if not _apart_or_same(x_out, x):
                     raise RuntimeError("rmsnorm: x_out is x or memory of its own")
                 ldo = _leading(x_out, cols, "x_out")
+                if _overlap(x_out, gamma):
+                    raise RuntimeError("rmsnorm: x_out must not overlap gamma")
             if not _apart_or_same(x_out, delta):
                 raise RuntimeError("rmsnorm: x_out is delta or memory of its own")
     return rows, cols, ldx, ldd, d_dtype, ldo, x_out, _launch_stream(x, gamma, delta, x_out)
@@ -1267,11 +1269,13 @@ def rmsnorm_fwd_fp8(x: torch.Tensor, gamma: torch.Tensor, delta: Optional[torch.
 
 def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dgamma_out: torch.Tensor,
                 dres: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """dx = dres + d rmsnorm / dx (dy); dgamma_out [cols] is written.  `x`: the normed stream, a tensor or the checkpoint the
-    forward left; rstd: the forward's.  dx has dres's dtype (dy's without one); `out` may be dres or dy."""
+    """dx = dres + d rmsnorm / dx (dy); dgamma_out [cols], memory of its own, is written.  `x`: the normed stream, a tensor or
+    the checkpoint the forward left; rstd: the forward's.  dx has dres's dtype (dy's without one); `out` may be dres or dy."""
     rows, cols, ldy = _row_layout(dy, "dy")
     _few_rows(rows)
     _vector(gamma, cols, "gamma"), _vector(rstd, rows, "rstd"), _vector(dgamma_out, cols, "dgamma_out")
+    if dgamma_out.data_ptr() in (gamma.data_ptr(), rstd.data_ptr()):
+        raise RuntimeError("rmsnorm_bwd: dgamma_out is memory of its own")
     q = code = None
     ldx = x_dtype = ldr = 0
     if isinstance(x, torch.Tensor):
@@ -1351,8 +1355,9 @@ def embed_scaled_bwd(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: 
         if accumulate:
             raise RuntimeError("accumulate needs an `out` to add into")
         out = dy.new_empty((vocab, cols), dtype=torch.float32)
-    elif out.dtype != torch.float32 or tuple(out.shape) != (vocab, cols) or not out.is_contiguous() or _overlap(out, dy):
-        raise RuntimeError(f"embed_scaled_bwd: out must be a contiguous float32 {(vocab, cols)} tensor apart from dy")
+    elif out.dtype != torch.float32 or tuple(out.shape) != (vocab, cols) or not out.is_contiguous() or _overlap(out, dy) \
+            or _overlap(out, tokens):
+        raise RuntimeError(f"embed_scaled_bwd: out must be a contiguous float32 {(vocab, cols)} tensor apart from dy and the ids")
     stream = _launch_stream(dy, tokens, out, err_flag)
     need = lib.bf_embed_scaled_bwd_workspace_bytes(n, cols, vocab)
     ws = dy.new_empty(need, dtype=torch.uint8) if need else None

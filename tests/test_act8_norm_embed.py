@@ -28,6 +28,7 @@ def test_act8_refusals(L):
     refused(L, lib.bf_act8_pack(PTR, 64, L.F32, PTR, None, 4, 64, None), -1, "null")
     refused(L, lib.bf_act8_pack(PTR + 2, 64, L.F32, PTR, PTR, 4, 64, None), -2, "aligned")
     refused(L, lib.bf_act8_pack(PTR, 32, L.F16, PTR, PTR, 1 << 30, 32, None), -1, "2^34")
+    refused(L, lib.bf_act8_pack(PTR, 128, L.F16, PTR, PTR, 1 << 60, 128, None), -1, "2^34")    # 2^60 rows of 2^4 vectors: 2^64
     refused(L, lib.bf_act8_unpack(PTR, PTR, PTR, 63, L.F16, 4, 64, None), -1, "leading dimension")
     refused(L, lib.bf_act8_unpack(PTR, PTR, PTR + 1, 64, L.F16, 4, 64, None), -2, "aligned")
     for act in (L.ACT_NONE, 3, 5, 99):
@@ -150,6 +151,13 @@ def test_wrappers_refuse_before_the_library(L):
         ops.rmsnorm_bwd(buf[:4], x, gamma, torch.ones(4), torch.empty(64), out=buf[1:])
     with pytest.raises(RuntimeError, match="must not overlap"):
         ops.rmsnorm_bwd(x, buf[:4], gamma, torch.ones(4), torch.empty(64), out=buf[1:])
+    both = torch.zeros(4 * 64 + 64)
+    with pytest.raises(RuntimeError, match="overlap gamma"):
+        ops.rmsnorm_fwd(x, both[200:264], torch.float32, delta=x, x_out=both[:256].view(4, 64))
+    for used in (0, 1):
+        with pytest.raises(RuntimeError, match="dgamma_out is memory of its own"):
+            g, r = torch.ones(64), torch.ones(64)
+            ops.rmsnorm_bwd(torch.zeros(64, 64), torch.zeros(64, 64), g, r, (g, r)[used])
     with pytest.raises(TypeError, match="int32"):
         ops.embed_scaled_fwd(ids.long(), x, 1.0)
     with pytest.raises(TypeError, match="err_flag"):
@@ -162,6 +170,8 @@ def test_wrappers_refuse_before_the_library(L):
         ops.embed_scaled_bwd(x, ids, 10, 1.0, accumulate=True)
     with pytest.raises(RuntimeError, match="apart from dy"):
         ops.embed_scaled_bwd(x, ids, 10, 1.0, out=torch.zeros(9, 64))
+    with pytest.raises(RuntimeError, match="and the ids"):
+        ops.embed_scaled_bwd(x, both[:4].view(torch.int32), 4, 1.0, out=both[:256].view(4, 64))
 
 
 def test_lora_checkpoint_values():
