@@ -18,8 +18,11 @@ enum { A8_PACK = 0, A8_UNPACK = 1, A8_FWD = 2, A8_BWD = 3 };
 // 0.5 x (1 + tanh) without its cancellation at negative x;  erf GELU x Phi(x).  Derivative of x s(u): s + x u' s (1 - s).
 // fp32 tensors take the accurate exponential and division; 16-bit ones v_exp / v_rcp (relative error some 2^-21, the
 // result is rounded to 2^-9 or 2^-12).  |x| is cut at 100 in the derivative (in fp32 it is 0 or 1 from there on), a NaN stays.
+template <int ACT> __device__ __forceinline__ float gate_at(float x) {
+    return ACT == BF_ACT_QUICK_GELU ? 1.702f * x : 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
+}
 template <int ACT, bool EXACT> __device__ __forceinline__ float gate(float x) {
-    const float u = ACT == BF_ACT_QUICK_GELU ? 1.702f * x : 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
+    const float u = gate_at<ACT>(x);
     if constexpr (EXACT) return 1.0f / (1.0f + expf(-u));
     else return __builtin_amdgcn_rcpf(1.0f + __expf(-u));
 }
@@ -38,11 +41,16 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float act_slope(float 
             return 0.5f * erfcf(-0.70710678118654752440f * x) + x * 0.39894228040143267794f * expf(-0.5f * x * x);
         else return erf_gelu_grad_fast(x);
     } else {
-        const float s = gate<ACT, EXACT>(x);
         const float du = ACT == BF_ACT_QUICK_GELU ? 1.702f : 1.5957691216057308f * fmaf(0.134145f * x, x, 1.0f);
-        // 1 - s as the gate of the other side where an fp32 result could show the cancellation
-        const float r = EXACT ? gate<ACT, EXACT>(-x) : 1.0f - s;
-        return fmaf(x * du, s * r, s);
+        if constexpr (EXACT) {
+            // s and 1 - s from one exponential, without the cancellation that an fp32 result could show: with v = e^-|u| the
+            // larger is 1 / (1 + v), the smaller v / (1 + v)
+            const float u = gate_at<ACT>(x), v = expf(-fabsf(u)), large = 1.0f / (1.0f + v), small = v * large;
+            return fmaf(x * du, large * small, u < 0.0f ? small : large);
+        } else {
+            const float s = gate<ACT, EXACT>(x), r = 1.0f - s;
+            return fmaf(x * du, s * r, s);
+        }
     }
 }
 
