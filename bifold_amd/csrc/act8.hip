@@ -26,9 +26,33 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float gate(float x) {
     if constexpr (EXACT) return 1.0f / (1.0f + expf(-u));
     else return __builtin_amdgcn_rcpf(1.0f + __expf(-u));
 }
+// Phi(-|x|) and e^(-x^2/2) in fp32, without branches; the GELU's value is right to 7 units of 2^-24, its slope's terms to 5
+// (73 728 x 768, forward 81 us, backward 83; with erfcf, whose lanes part at |x|, 89 and 93).  Phi(-a) = e^(-a^2/2) R(a); R(a) (a + 3.75) is smooth and bounded, here a polynomial of degree 8
+// in (a - 3.75) / (a + 3.75), fitted through Chebyshev nodes on 0 <= a <= 15 (4.2e-8 of the value).  a^2's rounding is made
+// good in the exponential.  From |x| = 15 on e^(-x^2/2) is under fp32's smallest number; |x| is cut at 20, where it is 0.
+__device__ __forceinline__ float normal_tail(float x, float& e) {
+    const float a = fminf(fabsf(x), 20.0f), h = a * a;
+    e = expf(-0.5f * h);
+    e = fmaf(e, -0.5f * fmaf(a, a, -h), e);
+    const float q = __builtin_amdgcn_rcpf(a + 3.75f), u = (a - 3.75f) * q;
+    float r = 4.4473037e-04f;
+    r = fmaf(r, u, 5.11906e-04f);
+    r = fmaf(r, u, -4.1687856e-03f);
+    r = fmaf(r, u, 1.198799e-03f);
+    r = fmaf(r, u, 3.7492145e-02f);
+    r = fmaf(r, u, -1.5152062e-01f);
+    r = fmaf(r, u, 3.5293967e-01f);
+    r = fmaf(r, u, -5.881883e-01f);
+    r = fmaf(r, u, 7.502941e-01f);
+    return e * (r * q);
+}
 template <int ACT, bool EXACT> __device__ __forceinline__ float act_value(float x) {
     if constexpr (ACT == BF_ACT_ERF_GELU) {
-        if constexpr (EXACT) return 0.5f * x * erfcf(-0.70710678118654752440f * x);
+        if constexpr (EXACT) {
+            float e;
+            const float t = normal_tail(x, e);
+            return x * (x < 0.0f ? t : 1.0f - t);
+        }
         else return erf_gelu_fast(x);
     } else {
         return x * gate<ACT, EXACT>(x);
@@ -37,8 +61,11 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float act_value(float 
 template <int ACT, bool EXACT> __device__ __forceinline__ float act_slope(float x) {
     x = fabsf(x) > 100.0f ? copysignf(100.0f, x) : x;
     if constexpr (ACT == BF_ACT_ERF_GELU) {
-        if constexpr (EXACT)
-            return 0.5f * erfcf(-0.70710678118654752440f * x) + x * 0.39894228040143267794f * expf(-0.5f * x * x);
+        if constexpr (EXACT) {
+            float e;
+            const float t = normal_tail(x, e);
+            return fmaf(x * 0.39894228040143267794f, e, x < 0.0f ? t : 1.0f - t);
+        }
         else return erf_gelu_grad_fast(x);
     } else {
         const float du = ACT == BF_ACT_QUICK_GELU ? 1.702f : 1.5957691216057308f * fmaf(0.134145f * x, x, 1.0f);
