@@ -27,9 +27,10 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float gate(float x) {
     else return __builtin_amdgcn_rcpf(1.0f + __expf(-u));
 }
 // Phi(-|x|) and e^(-x^2/2) in fp32, without branches; the GELU's value is right to 7 units of 2^-24, its slope's terms to 5
-// (73 728 x 768, forward 81 us, backward 83; with erfcf, whose lanes part at |x|, 89 and 93).  Phi(-a) = e^(-a^2/2) R(a); R(a) (a + 3.75) is smooth and bounded, here a polynomial of degree 8
-// in (a - 3.75) / (a + 3.75), fitted through Chebyshev nodes on 0 <= a <= 15 (4.2e-8 of the value).  a^2's rounding is made
-// good in the exponential.  From |x| = 15 on e^(-x^2/2) is under fp32's smallest number; |x| is cut at 20, where it is 0.
+// (73 728 x 768, forward 81 us, backward 83; with erfcf, whose lanes part at |x|, 89 and 93).  Phi(-a) = e^(-a^2/2) R(a), and
+// R(a) (a + 3.75) is smooth and bounded: a polynomial of degree 8 in (a - 3.75) / (a + 3.75), fitted through Chebyshev nodes on
+// 0 <= a <= 15 to 4.2e-8 of the value.  The rounding of a^2 is made good behind the exponential.  From |x| = 15 on e^(-x^2/2)
+// is under fp32's smallest number; |x| is cut at 20, where it is 0.
 __device__ __forceinline__ float normal_tail(float x, float& e) {
     const float a = fminf(fabsf(x), 20.0f), h = a * a;
     e = expf(-0.5f * h);
