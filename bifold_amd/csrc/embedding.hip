@@ -56,11 +56,13 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
 // smaller digits, of earlier tiles and of earlier waves -- and moves its tokens.  (Counting the next pass's digits by global
 // atomics while moving saves a launch and costs more: 131 072 tokens 74 instead of 59 us.)  Digits of up to 9 bits put a
 // vocabulary of 2^18 into two passes.  Ids outside the table and the padding token become the key `vocab`, which sorts
-// behind the others.  131 072 tokens take 28 us, 8 192 take 15: four short dependent launches, bound by their latencies.
+// behind the others.  131 072 tokens take 28 us in four short dependent launches, bound by their latencies; few tokens need
+// no count launch (embed_scatter_kernel): 8 192 take 11.6 us, with them 14.6.
 #define SORT_THREADS 512
 #define SORT_WAVES 8
 #define SORT_MAX_BINS 512
 #define SORT_MAX_TILES 64
+#define SORT_SELF 12288                         /* tokens; a digit's counts are kept in 16 bits */
 
 struct SortArgs {
     const int32_t* ids; int n; int vocab; int pad;
@@ -82,15 +84,18 @@ __device__ __forceinline__ int2 sort_item(const SortArgs& a, int i, int* err_fla
         return a.in[i];
     }
 }
-template <bool FIRST>
-__global__ __launch_bounds__(SORT_THREADS) void embed_hist_kernel(const SortArgs a) {
-    __shared__ int bins[SORT_MAX_BINS];
-    if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) *a.owner_count = 0;
-    if (FIRST && a.present) {
+__device__ __forceinline__ void sort_clear(const SortArgs& a) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.owner_count = 0;
+    if (a.present) {
         unsigned* words = (unsigned*)a.present;
         const int many = (int)(((unsigned)a.vocab + 3u) >> 2);
         for (int i = blockIdx.x * SORT_THREADS + threadIdx.x; i < many; i += a.tiles * SORT_THREADS) words[i] = 0;
     }
+}
+template <bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void embed_hist_kernel(const SortArgs a) {
+    __shared__ int bins[SORT_MAX_BINS];
+    if (FIRST) sort_clear(a);
     bins[threadIdx.x] = 0;
     __syncthreads();
     const int base = blockIdx.x * SORT_THREADS * a.rounds, mask = (1 << a.dbits) - 1;
@@ -101,14 +106,25 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_hist_kernel(const SortArgs
     __syncthreads();
     a.hist[blockIdx.x * SORT_MAX_BINS + threadIdx.x] = bins[threadIdx.x];
 }
-template <bool FIRST>
+// SELF: no count launch, every workgroup counts all tokens itself.  The whole gradient of n tokens x 64 fp16, added, with and
+// without: 2 049 21 and 25 us, 4 096 22 and 25, 8 192 26 and 28, 12 288 28 and 30, 16 384 36 and 36, so up to 12 288 tokens.
+template <bool FIRST, bool SELF>
 __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortArgs a) {
     __shared__ int cnt[SORT_WAVES][SORT_MAX_BINS];
     __shared__ int wave_tot[SORT_WAVES];
+    // lanes of one digit wait for each other at its counter, and padding makes one token frequent: copies on different banks
+    // (8 192 times one token: 25 us with 8, 29 with 2, 35 with one)
+    constexpr int COPIES = 8, SKEW = 4;
+    __shared__ unsigned all[SELF ? COPIES * (SORT_MAX_BINS + SKEW) : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int mask = (1 << a.dbits) - 1, span = SORT_THREADS * a.rounds;
 #pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) cnt[w][tid] = 0;
+    if constexpr (SELF) {
+#pragma unroll
+        for (int k = 0; k < COPIES; ++k) all[k * (SORT_MAX_BINS + SKEW) + tid] = 0;
+        if (FIRST) sort_clear(a);
+    }
     __syncthreads();
     // a wave owns `rounds` x 64 consecutive tokens of the tile
     const int first = blockIdx.x * span + wave * 64 * a.rounds + lane;
@@ -119,7 +135,27 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
     }
     // all tokens of this thread's digit, and those in earlier tiles: sixteen tiles' counts in flight
     int tot = 0, before = 0;
-    for (int t0 = 0; t0 < a.tiles; t0 += 16) {
+    if constexpr (SELF) {                       // a digit's tokens in the low half of a word, those in earlier tiles in the high
+        const int start = blockIdx.x * span;
+        unsigned* const copy = all + (lane & (COPIES - 1)) * (SORT_MAX_BINS + SKEW);
+        for (int i0 = tid; i0 < a.n; i0 += 8 * SORT_THREADS) {
+            int key[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) key[u] = sort_item<FIRST>(a, min(i0 + u * SORT_THREADS, a.n - 1), nullptr).x;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * SORT_THREADS;
+                if (i < a.n) atomicAdd(&copy[(key[u] >> a.shift) & mask], i < start ? 0x10001u : 1u);
+            }
+        }
+        __syncthreads();
+        unsigned both = 0;
+#pragma unroll
+        for (int k = 0; k < COPIES; ++k) both += all[k * (SORT_MAX_BINS + SKEW) + tid];
+        tot = (int)(both & 0xFFFFu);
+        before = (int)(both >> 16);
+    }
+    for (int t0 = 0; !SELF && t0 < a.tiles; t0 += 16) {
         int h[16];
 #pragma unroll
         for (int u = 0; u < 16; ++u) h[u] = a.hist[min(t0 + u, a.tiles - 1) * SORT_MAX_BINS + tid];
@@ -150,12 +186,13 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
     // by a ballot per digit bit; the first of them moves the place on.  LDS accesses of one wave complete in order; the
     // relaxed atomics keep the compiler from holding a place in a register.
     int* mine = cnt[wave];
-    int2 item = first < a.n ? sort_item<FIRST>(a, first, nullptr) : make_int2(0, 0);
+    int* const flag = SELF ? a.err_flag : nullptr;
+    int2 item = first < a.n ? sort_item<FIRST>(a, first, flag) : make_int2(0, 0);
     for (int r = 0; r < a.rounds; ++r) {
         const int i = first + r * 64;
         const bool live = i < a.n;
         const int2 it = item;
-        if (r + 1 < a.rounds && i + 64 < a.n) item = sort_item<FIRST>(a, i + 64, nullptr);
+        if (r + 1 < a.rounds && i + 64 < a.n) item = sort_item<FIRST>(a, i + 64, flag);
         const int d = (it.x >> a.shift) & mask;
         unsigned long long same = __ballot(live);
         for (int b = 0; b < a.dbits; ++b) {
@@ -168,14 +205,15 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
             const int at = __hip_atomic_load(&mine[d], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
             a.out[at + rank] = it;
             if (rank == 0) __hip_atomic_store(&mine[d], at + __popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-            if (FIRST && a.present && it.x < a.vocab) a.present[it.x] = 1;     // whoever stores it, it is the same byte
+            // whoever stores it, it is the same byte; a launch after the one that cleared the table
+            if (FIRST != SELF && a.present && it.x < a.vocab) a.present[it.x] = 1;
         }
     }
 }
 
 // Up to 2 048 tokens of a vocabulary under 2^18: the same sort by one workgroup, in LDS, one launch (the whole gradient of
-// 2 048 x 1 024 fp32, added into one that is there: 18 instead of 24 us; 4 096 tokens 24 and 26, 8 192 37 and 33: one CU is
-// not enough there).  A token is one word, its key over its place (11 bits; a larger vocabulary would fit, but one workgroup
+// 2 048 x 64 fp16, added into one that is there: 19 us instead of 22, of 1 024 17.5 instead of 20.5; 8 192 x 1 024 fp32 37
+// instead of 31: one CU is not enough there).  A token is one word, its key over its place (11 bits; a larger vocabulary would fit, but one workgroup
 // also clears its table of bytes); a thread holds R of them, a wave R x 64 consecutive ones.  Places behind the last token
 // hold the largest word, which stays behind.
 #define ONE_THREADS 1024
@@ -527,7 +565,7 @@ __global__ __launch_bounds__(FEW) void embed_few_kernel(const int32_t* __restric
 
 // ------------------------------------------------------------------ plan of a call
 struct EmbedPlan {
-    bool one;                                   // sorted by one workgroup
+    bool one, self;                             // sorted by one workgroup; without count launches
     int passes, dbits, rounds, tiles, chunk, chunks;
     size_t pairs, hist, owners, present, part, bytes;            // offsets into the workspace
 };
@@ -538,6 +576,7 @@ EmbedPlan embed_plan(int n, int cols, int vocab) {
     p.one = n <= ONE_MAX && vocab < (1 << 18);
     p.passes = p.one ? (bits + 7) / 8 : (bits + 8) / 9;          // digits of up to 8 or 9 bits
     p.dbits = (bits + p.passes - 1) / p.passes;
+    p.self = !p.one && p.passes > 1 && n <= SORT_SELF;           // the first pass clears the table of bytes, later ones mark
     const long span = (long)SORT_THREADS * SORT_MAX_TILES;
     p.rounds = (int)((n + span - 1) / span);
     p.tiles = (n + SORT_THREADS * p.rounds - 1) / (SORT_THREADS * p.rounds);
@@ -689,12 +728,15 @@ extern "C" int bf_embed_scaled_bwd(const void* dy, int64_t ld_dy, int dy_dtype, 
             q.shift = pass * p.dbits;
             q.in = pairs[(pass + 1) & 1];
             q.out = pairs[pass & 1];
-            if (pass == 0) {
+            if (p.self) {
+                if (pass == 0) hipLaunchKernelGGL((embed_scatter_kernel<true, true>), grid, block, 0, s, q);
+                else hipLaunchKernelGGL((embed_scatter_kernel<false, true>), grid, block, 0, s, q);
+            } else if (pass == 0) {
                 hipLaunchKernelGGL((embed_hist_kernel<true>), grid, block, 0, s, q);
-                hipLaunchKernelGGL((embed_scatter_kernel<true>), grid, block, 0, s, q);
+                hipLaunchKernelGGL((embed_scatter_kernel<true, false>), grid, block, 0, s, q);
             } else {
                 hipLaunchKernelGGL((embed_hist_kernel<false>), grid, block, 0, s, q);
-                hipLaunchKernelGGL((embed_scatter_kernel<false>), grid, block, 0, s, q);
+                hipLaunchKernelGGL((embed_scatter_kernel<false, false>), grid, block, 0, s, q);
             }
             BF_CHECK_LAUNCH(name);
         }

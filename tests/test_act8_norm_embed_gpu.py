@@ -403,7 +403,7 @@ def tokens_of(kind, n, vocab, g):
 
 EMBEDS = [(1, 1, 1), (1, 64, 100), (2, 7, 3), (77, 512, 49408), (300, 33, 1000), (511, 520, 50), (512, 1100, 300), (513, 16, 200),
           (700, 1030, 513), (1000, 64, 1), (1024, 2100, 90), (1025, 520, 30), (1500, 7, 40), (2000, 12, 2_100_000), (2048, 72, 70000), (2049, 72, 300), (4096, 40, 32000), (5000, 768, 511), (9000, 24, 300000), (20000, 72, 65536), (70000, 8, 600),
-          (33000, 520, 20), (16601, 1024, 300)]
+          (33000, 520, 20), (16601, 1024, 300), (12288, 16, 1000), (12289, 16, 600), (2100, 9, 511), (2100, 9, 512)]
 
 
 @pytest.mark.parametrize("n,cols,vocab", EMBEDS)
