@@ -212,8 +212,8 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(const SortA
 }
 
 // Up to 2 048 tokens of a vocabulary under 2^18: the same sort by one workgroup, in LDS, one launch (the whole gradient of
-// 2 048 x 64 fp16, added into one that is there: 19 us instead of 22, of 1 024 17.5 instead of 20.5; 8 192 x 1 024 fp32 37
-// instead of 31: one CU is not enough there).  A token is one word, its key over its place (11 bits; a larger vocabulary would fit, but one workgroup
+// 2 048 x 64 fp16, added into one that is there: 19 us instead of 22, of 1 024 17.5 instead of 20.5; 8 192 x 1 024 fp32 37,
+// by four launches 33: one CU is not enough there).  A token is one word, its key over its place (11 bits; a larger vocabulary would fit, but one workgroup
 // also clears its table of bytes); a thread holds R of them, a wave R x 64 consecutive ones.  Places behind the last token
 // hold the largest word, which stays behind.
 #define ONE_THREADS 1024
