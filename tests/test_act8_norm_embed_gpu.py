@@ -722,3 +722,39 @@ def test_lora_backward_from_checkpoints(ops, gpu, dtype, p_drop, policy):
         assert torch.equal(seen["int8"][1][n], gr), n
         assert torch.isfinite(gr).all() and gr.abs().max() > 0
     assert any(not torch.equal(seen["int8"][1][n], gr) for n, gr in seen["native"][1].items())
+
+
+# ------------------------------------------------------------------ the erf GELU's digits far below zero
+def erf_gelu_ref(x):
+    """(x Phi(x), Phi(x), x phi(x)) in 64 bits; erfc keeps its digits at any x < 0."""
+    cdf = 0.5 * torch.erfc(-x / math.sqrt(2))
+    return x * cdf, cdf, x * torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+
+
+# 16-bit tensors: the exponential's argument is a product with a rounded log2(e), U |x^2| together at most; the polynomial's fit
+# (13 U) and evaluation (7 U), reciprocal, exponential and products add less than 32 U; the result is rounded to the type.  An exponential under fp32's
+# smallest normal number, 2^-126, may be 0, and Phi(-x) and x phi(x) are under 0.03 and 6 times it there (13 < x < 14).
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_act8_erf_gelu_of_every_16_bit_value(ops, L, gpu, dtype):
+    x = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x[torch.isfinite(x) & (x.abs() <= 14)]
+    x = torch.cat([x, torch.zeros(-len(x) % 64, dtype=dtype)]).view(-1, 64)
+    y, _ = ops.act8_gelu_fwd(x.to(gpu), L.ACT_ERF_GELU)
+    ref = x.double()
+    want, _, _ = erf_gelu_ref(ref)
+    bound = want.abs() * (half_step(dtype) + (ref * ref + 32) * U) + tiny_step(dtype)
+    close(y, want, bound + torch.where(ref < -13, 2.0 ** -126, 0.0), "y")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_act8_erf_gelu_slope_of_every_kept_value(ops, L, gpu, dtype):
+    """Checkpoints q 2^e as they can be: every q, steps 2^-12 to 2^-3."""
+    q = torch.arange(-127, 128, dtype=torch.int8)
+    q = torch.cat([q, q[:1]]).view(8, 32).repeat(10, 1).contiguous()
+    code = torch.arange(115, 125, dtype=torch.uint8).repeat_interleave(8).view(-1, 1)
+    at = q.double() * torch.exp2(code.double() - 127)
+    slope = ops.act8_gelu_bwd(torch.ones(80, 32, dtype=dtype, device=gpu), (q.to(gpu), code.to(gpu)), L.ACT_ERF_GELU)
+    _, cdf, part = erf_gelu_ref(at)
+    want = cdf + part
+    bound = want.abs() * half_step(dtype) + (cdf + part.abs()) * (at * at + 32) * U + tiny_step(dtype)
+    close(slope, want, bound + torch.where(at < -13, 6 * 2.0 ** -126, 0.0), "slope")
