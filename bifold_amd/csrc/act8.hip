@@ -116,7 +116,8 @@ __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
     size_t off_x, off_y, off_q, off_c;
     bool first;
     if constexpr (A == ROWS_ALIGNED) {
-        n = live ? V : 0;
+        if (MODE == A8_UNPACK && !live) return;                // no lane needs another: one branch around everything
+        n = MODE == A8_UNPACK || live ? V : 0;
         off_x = off_y = off_q = (size_t)v * V;
         off_c = v / PER;
         first = v % PER == 0;
@@ -153,6 +154,14 @@ __global__ __launch_bounds__(256) void act8_kernel(const A8Args a) {
         if constexpr (MODE == A8_BWD) dy.template load<true>(x, 0, n);
         q.words(w, n);
         act8_dequant<V>(w, code, f);
+        if constexpr (MODE == A8_UNPACK && __is_same(T, f16_t)) {
+            // 2^16 is what fp16's numbers from 65 280 on are kept as, and the one value of theirs that fp16 does not hold; a wave
+            // seldom has a step of 2^10 or more
+            if (__ballot(code >= 137u) != 0) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) f[j] = fabsf(f[j]) == 65536.0f ? copysignf(65504.0f, f[j]) : f[j];
+            }
+        }
         if constexpr (MODE == A8_BWD) {
             float d[V];
             dy.take(d, n);

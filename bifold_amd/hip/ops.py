@@ -1160,7 +1160,9 @@ def act8_pack(x: torch.Tensor) -> Checkpoint:
 
 
 def act8_unpack(kept: Checkpoint, dtype: torch.dtype, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The tensor a checkpoint stands for: q 2^e (exact in fp32 and bf16; NaN throughout a group that was not finite)."""
+    """The tensor a checkpoint stands for: q 2^e (exact in fp32, bf16 and fp16, except that fp16 takes 2^16, as which its
+    numbers from 65 280 on are kept, as 65 504).  NaN throughout a group that held a NaN, an infinity or a magnitude of
+    255 * 2^119 or more."""
     q, code = _act8_parts(kept)
     if out is None:
         out = _like(q, dtype)

@@ -655,7 +655,8 @@ int bf_gaussian_targets(const float* points, const int32_t* counts, float* heat,
  *   shares the power of two 2^e, e the smallest exponent >= -126 for which round(max |x| 2^-e) <= 127;
  *     q [rows, cols] int8 = round(x 2^-e), ties to even      code [rows, ceil(cols / 32)] uint8 = e + 127
  *   and x reads back as q 2^e: off by at most 2^(e-1) <= max |x| / 127.  A group with a NaN, an infinity or a magnitude of
- *   255 * 2^119 or more has code 255 and reads back as NaN.
+ *   255 * 2^119 or more has code 255 and reads back as NaN.  Unpacking to BF_F16 writes +-2^16, which fp16's numbers from
+ *   65 280 on are kept as, as +-65 504 (larger values, from wider types, as infinities).
  * dtype: BF_F32 / BF_BF16 / BF_F16 of x, pre, y, dy, dpre.  rows * ceil(cols / 32) < 2^29.  Pointers need the alignment
  * of their element only; cols a multiple of 32, no gaps between rows and 16-byte alignment give the fast path.
  *   gelu_fwd: y [rows, cols] = act(pre) and the checkpoint of pre, one pass.  act: BF_ACT_QUICK_GELU / _ERF_GELU / _TANH_GELU

@@ -758,3 +758,27 @@ def test_act8_erf_gelu_slope_of_every_kept_value(ops, L, gpu, dtype):
     want = cdf + part
     bound = want.abs() * half_step(dtype) + (cdf + part.abs()) * (at * at + 32) * U + tiny_step(dtype)
     close(slope, want, bound + torch.where(at < -13, 6 * 2.0 ** -126, 0.0), "slope")
+
+
+# ------------------------------------------------------------------ fp16's largest numbers
+@pytest.mark.parametrize("cols", [7, 32, 45, 96])
+def test_finite_fp16_reads_back_finite(ops, gpu, cols):
+    """65 280 (255 * 2^8) and above are kept as 64 * 2^10 = 2^16, which fp16 does not hold; a step of 2^10 is off by 2^9 at most."""
+    top = torch.finfo(torch.float16).max
+    x = torch.zeros(6, cols, dtype=torch.float16)
+    x[0, 0], x[0, 1] = top, 1024.0
+    x[1, cols - 1], x[1, 0] = -top, 3.0
+    x[2, 3] = 65280.0
+    x[3, 3] = 65248.0                                           # the largest number that is not kept as 2^16
+    x[4, 0], x[4, cols - 1] = 65472.0, -65312.0
+    x[5, 1] = math.inf
+    kept = ops.act8_pack(x.to(gpu))
+    back = ops.act8_unpack(kept, torch.float16).cpu()
+    assert torch.isfinite(back[:5]).all() and back[5, :32].isnan().all()
+    assert (back[:5].double() - x[:5].double()).abs().max() <= 512
+    assert back[0, :2].tolist() == [top, 1024.0] and back[1, cols - 1] == -top and back[2, 3] == top and back[3, 3] == 65024.0
+    wide = ops.act8_unpack(kept, torch.float32).cpu()           # a wider type holds what is kept
+    assert wide[0, 0] == 65536.0 and wide[1, cols - 1] == -65536.0
+    far = torch.zeros(1, cols)
+    far[0, 0], far[0, 1] = 1e5, -1e5                            # no fp16 number: an overflow stays one
+    assert ops.act8_unpack(ops.act8_pack(far.to(gpu)), torch.float16)[0, :2].tolist() == [math.inf, -math.inf]
