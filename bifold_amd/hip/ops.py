@@ -1276,8 +1276,6 @@ def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dg
     rows, cols, ldy = _row_layout(dy, "dy")
     _few_rows(rows)
     _vector(gamma, cols, "gamma"), _vector(rstd, rows, "rstd"), _vector(dgamma_out, cols, "dgamma_out")
-    if dgamma_out.data_ptr() in (gamma.data_ptr(), rstd.data_ptr()):
-        raise RuntimeError("rmsnorm_bwd: dgamma_out is memory of its own")
     q = code = None
     ldx = x_dtype = ldr = 0
     if isinstance(x, torch.Tensor):
@@ -1303,6 +1301,13 @@ def rmsnorm_bwd(dy: torch.Tensor, x, gamma: torch.Tensor, rstd: torch.Tensor, dg
         for t in (x, q, code, gamma, rstd, dgamma_out):
             if t is not None and _overlap(out, t):
                 raise RuntimeError("rmsnorm_bwd: out must not overlap x, the checkpoint, gamma, rstd or dgamma_out")
+    first = dgamma_out.data_ptr()
+    end = first + 4 * cols
+    for t in (dy, x, q, code, gamma, rstd, dres):
+        if t is not None:
+            at = t.data_ptr()
+            if at < end and (at >= first or at + t.nbytes > first or not t.is_contiguous()) and _overlap(dgamma_out, t):
+                raise RuntimeError("rmsnorm_bwd: dgamma_out is memory of its own")
     stream = _launch_stream(dy, x, q, code, gamma, rstd, dres, out, dgamma_out)
     parts = gamma.new_empty(lib.bf_rmsnorm_bwd_parts(rows, cols) * cols)
     check(lib.bf_rmsnorm_bwd(dy.data_ptr(), ldy, dtype_code(dy), _ptr(x), ldx, x_dtype, _ptr(q), _ptr(code), gamma.data_ptr(),

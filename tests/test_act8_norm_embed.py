@@ -183,3 +183,37 @@ def test_lora_checkpoint_values():
     assert SiglipTowers(vision, text, lora=dict(lora, checkpoint="int8")).lora["checkpoint"] == "int8"
     with pytest.raises(ValueError, match="native or int8"):
         SiglipTowers(vision, text, lora=dict(lora, checkpoint="int4"))
+
+
+def test_norm_gradient_over_an_operand_is_refused(L):
+    """dgamma_out is written while other workgroups still read, so it overlaps no operand, in part or whole."""
+    from bifold_amd.hip import ops
+    rows, cols = 4, 64
+
+    def bwd(dg, dy=None, x=None, gamma=None, rstd=None, dres=None):
+        return ops.rmsnorm_bwd(torch.zeros(rows, cols) if dy is None else dy, torch.zeros(rows, cols) if x is None else x,
+                               torch.ones(cols) if gamma is None else gamma, torch.ones(rows) if rstd is None else rstd, dg, dres=dres)
+
+    flat = torch.zeros((rows + 1) * cols)
+    rows_of = flat[:rows * cols].view(rows, cols)
+    wide = torch.zeros(rows, 2 * cols)
+    mine = "dgamma_out is memory of its own"
+    for dg in (flat[:cols], flat[100:100 + cols], flat[rows * cols - 1:(rows + 1) * cols - 1]):
+        for name in ("dy", "x", "dres"):
+            with pytest.raises(RuntimeError, match=mine):
+                bwd(dg, **{name: rows_of})
+    for name in ("dy", "x", "dres"):                              # a view that starts in front of dgamma_out and ends behind it
+        with pytest.raises(RuntimeError, match=mine):
+            bwd(wide[2, 8:8 + cols], **{name: wide[:, :cols]})
+    with pytest.raises(RuntimeError, match=mine):
+        bwd(flat[1:1 + cols], gamma=flat[:cols])
+    with pytest.raises(RuntimeError, match=mine):
+        bwd(flat[:cols], rstd=flat[60:64])
+    q, code = flat[:rows * cols // 4].view(torch.int8).view(rows, cols), torch.ones(rows, 2, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match=mine):
+        bwd(flat[8:8 + cols], x=(q, code))
+    big = torch.zeros(2 * cols)
+    with pytest.raises(RuntimeError, match=mine):
+        bwd(big[:cols], x=(torch.zeros(rows, cols, dtype=torch.int8), big.view(torch.uint8)[12:20].view(rows, 2)))
+    with pytest.raises(RuntimeError, match="no CPU path"):        # next to its operands: nothing to refuse but the device
+        bwd(flat[rows * cols:], dy=rows_of, gamma=big[:cols], dres=None)
