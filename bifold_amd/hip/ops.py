@@ -1230,8 +1230,8 @@ def _rms_args(x, gamma, delta, x_out, write_x):
                 if not _apart_or_same(x_out, x):
                     raise RuntimeError("rmsnorm: x_out is x or memory of its own")
                 ldo = _leading(x_out, cols, "x_out")
-                if -4 * cols < gamma.data_ptr() - x_out.data_ptr() < ((rows - 1) * ldo + cols) * x_out.element_size():
-                    raise RuntimeError("rmsnorm: x_out must not overlap gamma")
+            if -4 * cols < gamma.data_ptr() - x_out.data_ptr() < ((rows - 1) * ldo + cols) * x_out.element_size():
+                raise RuntimeError("rmsnorm: x_out must not overlap gamma")
             if not _apart_or_same(x_out, delta):
                 raise RuntimeError("rmsnorm: x_out is delta or memory of its own")
     return rows, cols, ldx, ldd, d_dtype, ldo, x_out, _launch_stream(x, gamma, delta, x_out)

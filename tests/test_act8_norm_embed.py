@@ -217,3 +217,20 @@ def test_norm_gradient_over_an_operand_is_refused(L):
         bwd(big[:cols], x=(torch.zeros(rows, cols, dtype=torch.int8), big.view(torch.uint8)[12:20].view(rows, 2)))
     with pytest.raises(RuntimeError, match="no CPU path"):        # next to its operands: nothing to refuse but the device
         bwd(flat[rows * cols:], dy=rows_of, gamma=big[:cols], dres=None)
+
+
+def test_norm_in_place_over_gamma_is_refused(L):
+    """x += delta in place, with gamma inside x: rows would be scaled by what others have already written."""
+    from bifold_amd.hip import ops
+    flat = torch.zeros(5 * 64)
+    x, delta = flat[:256].view(4, 64), torch.zeros(4, 64)
+    for gamma in (flat[:64], flat[100:164], flat[255:319]):
+        for out in (None, x):
+            with pytest.raises(RuntimeError, match="must not overlap gamma"):
+                ops.rmsnorm_fwd(x, gamma, torch.float32, delta=delta, x_out=out)
+            with pytest.raises(RuntimeError, match="must not overlap gamma"):
+                ops.rmsnorm_fwd_fp8(x, gamma, delta=delta, x_out=out)
+    for call in (lambda: ops.rmsnorm_fwd(x, flat[256:], torch.float32, delta=delta),
+                 lambda: ops.rmsnorm_fwd(x, flat[:64], torch.float32, delta=delta, write_x=False)):      # read only
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
