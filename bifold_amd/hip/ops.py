@@ -1111,15 +1111,24 @@ def _vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Do the address ranges of two tensors meet?  (Strided views count from their first to their last element.)"""
+    """Do two tensors share memory?  2-D views whose rows are equally far apart (columns of one buffer) are compared row by
+    row, others by their ranges from the first to the last element."""
     pa, pb = a.data_ptr(), b.data_ptr()
     if a.is_contiguous() and b.is_contiguous():
         na, nb = a.nbytes, b.nbytes
-    else:
-        if a.numel() == 0 or b.numel() == 0:
-            return False
-        na, nb = ((sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b))
-    return pa < pb + nb and pb < pa + na and na > 0 and nb > 0
+        return pa < pb + nb and pb < pa + na and na > 0 and nb > 0
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    ea, eb = a.element_size(), b.element_size()
+    na, nb = ((sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * e for t, e in ((a, ea), (b, eb)))
+    if pa >= pb + nb or pb >= pa + na:
+        return False
+    if a.dim() == b.dim() == 2 and a.stride(1) == b.stride(1) == 1 and a.stride(0) * ea == b.stride(0) * eb:
+        step, wa, wb = a.stride(0) * ea, a.shape[1] * ea, b.shape[1] * eb
+        # b's rows begin `off` bytes behind one of a's and end in front of the next
+        off = (pb - pa) % step if step >= max(wa, wb) else 0
+        return off < wa or off + wb > step
+    return True
 
 
 def _apart_or_same(a: torch.Tensor, b: torch.Tensor) -> bool:

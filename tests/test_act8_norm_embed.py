@@ -234,3 +234,54 @@ def test_norm_in_place_over_gamma_is_refused(L):
                  lambda: ops.rmsnorm_fwd(x, flat[:64], torch.float32, delta=delta, write_x=False)):      # read only
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def test_columns_of_one_buffer_are_memory_of_their_own(L):
+    """Outputs beside their inputs in one packed buffer share no element with them, and are taken."""
+    from bifold_amd.hip import ops
+    wide = torch.zeros(4, 3 * 64)
+    left, mid, right = wide[:, :64], wide[:, 64:128], wide[:, 128:]
+    gamma, kept = torch.ones(64), (torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4, 2, dtype=torch.uint8))
+    for out in (left, right):
+        for call in (lambda: ops.act8_gelu_bwd(mid, kept, L.ACT_ERF_GELU, out=out),
+                     lambda: ops.rmsnorm_fwd(mid, gamma, torch.float32, delta=torch.zeros(4, 64), x_out=out),
+                     lambda: ops.rmsnorm_fwd(torch.zeros(4, 64), gamma, torch.float32, delta=mid, x_out=out)):
+            with pytest.raises(RuntimeError, match="no CPU path"):
+                call()
+    for out in (wide[:, 63:127], wide[:, 65:129], wide[:, 127:191], wide[:, 1:65]):
+        with pytest.raises(RuntimeError, match="memory of its own"):
+            ops.act8_gelu_bwd(mid, kept, L.ACT_ERF_GELU, out=out)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_overlap_against_the_addresses(L, seed):
+    """Views of one buffer share memory exactly where a set of their bytes says so; other layouts are never missed."""
+    import random
+    from bifold_amd.hip import ops
+    rng = random.Random(seed)
+    buf = torch.zeros(400, dtype=torch.uint8)
+
+    def view():
+        dtype = rng.choice([torch.uint8, torch.float16, torch.float32])
+        flat = buf.view(dtype)
+        rows, cols = rng.randint(0, 5), rng.randint(1, 9)
+        step = rng.choice([cols, rng.randint(cols, 20), 40 // flat.element_size()])
+        step = max(step, cols)
+        first = rng.randint(0, len(flat) - max(0, rows - 1) * step - cols)
+        return flat.as_strided((rows, cols), (step, 1), first)
+
+    def bytes_of(t):
+        base, e = t.data_ptr() - buf.data_ptr(), t.element_size()
+        return {base + (i * t.stride(0) + j) * e + k for i in range(t.shape[0]) for j in range(t.shape[1]) for k in range(e)}
+
+    exact = 0
+    for _ in range(3000):
+        a, b = view(), view()
+        meet, says = bool(bytes_of(a) & bytes_of(b)), ops._overlap(a, b)
+        assert says == ops._overlap(b, a)
+        if a.stride(0) * a.element_size() == b.stride(0) * b.element_size() and (a.shape[0] > 1 or b.shape[0] > 1):
+            exact += not meet and not (a.is_contiguous() and b.is_contiguous())
+            far = a.shape[0] <= 1 or b.shape[0] <= 1
+            assert says == meet or (far and says)
+        assert says or not meet, (a.shape, a.stride(), b.shape, b.stride())
+    assert exact > 20

@@ -782,3 +782,26 @@ def test_finite_fp16_reads_back_finite(ops, gpu, cols):
     far = torch.zeros(1, cols)
     far[0, 0], far[0, 1] = 1e5, -1e5                            # no fp16 number: an overflow stays one
     assert ops.act8_unpack(ops.act8_pack(far.to(gpu)), torch.float16)[0, :2].tolist() == [math.inf, -math.inf]
+
+
+# ------------------------------------------------------------------ outputs in the columns beside their inputs
+@pytest.mark.parametrize("cols,wide", [(64, 192), (37, 120), (7, 23), (1155, 3500), (17000, 51003)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_outputs_in_columns_of_the_inputs_buffer(ops, L, gpu, cols, wide, dtype):
+    """dy, dpre, the stream and the sum in one packed buffer: the same bits as apart, and the other columns untouched."""
+    rows = 9
+    buf = make(rows, wide, dtype, cols)[0]
+    before = buf.clone()
+    src, dst = buf[:, cols:2 * cols], buf[:, 2 * cols:3 * cols]
+    kept = ops.act8_pack(src.contiguous())
+    want = ops.act8_gelu_bwd(src.contiguous(), kept, L.ACT_TANH_GELU)
+    assert ops.act8_gelu_bwd(src, kept, L.ACT_TANH_GELU, out=dst) is dst
+    assert torch.equal(dst, want) and torch.equal(buf[:, :2 * cols], before[:, :2 * cols])
+    assert torch.equal(buf[:, 3 * cols:], before[:, 3 * cols:])
+    buf.copy_(before)
+    gamma, delta = 1 + torch.rand(cols, device=gpu), buf[:, :cols]
+    total = torch.empty(rows, cols, dtype=dtype, device=gpu)
+    want, _, _ = ops.rmsnorm_fwd(src.contiguous(), gamma, dtype, delta=delta.contiguous(), x_out=total)
+    y, _, _ = ops.rmsnorm_fwd(src, gamma, dtype, delta=delta, x_out=dst)
+    assert torch.equal(y, want) and torch.equal(dst, total) and torch.equal(buf[:, :2 * cols], before[:, :2 * cols])
+    assert torch.equal(buf[:, 3 * cols:], before[:, 3 * cols:])
