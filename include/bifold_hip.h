@@ -657,7 +657,7 @@ int bf_gaussian_targets(const float* points, const int32_t* counts, float* heat,
  *   and x reads back as q 2^e: off by at most 2^(e-1) <= max |x| / 127.  A group with a NaN, an infinity or a magnitude of
  *   255 * 2^119 or more has code 255 and reads back as NaN.  Unpacking to BF_F16 writes +-2^16, which fp16's numbers from
  *   65 280 on are kept as, as +-65 504 (larger values, from wider types, as infinities).
- * dtype: BF_F32 / BF_BF16 / BF_F16 of x, pre, y, dy, dpre.  rows * ceil(cols / 32) < 2^29.  Pointers need the alignment
+ * dtype: BF_F32 / BF_BF16 / BF_F16 of x, pre, y, dy, dpre.  rows * ceil(cols / 32) <= 2^29 - 1024.  Pointers need the alignment
  * of their element only; cols a multiple of 32, no gaps between rows and 16-byte alignment give the fast path.
  *   gelu_fwd: y [rows, cols] = act(pre) and the checkpoint of pre, one pass.  act: BF_ACT_QUICK_GELU / _ERF_GELU / _TANH_GELU
  *   gelu_bwd: dpre = dy act'(q 2^e); dpre may be dy (same leading dimension).
@@ -690,13 +690,15 @@ int bf_rmsnorm_bwd(const void* dy, int64_t ld_dy, int dy_dtype, const void* x, i
                    int dx_dtype, float* dgamma, float* parts_ws, int rows, int cols, bf_stream_t stream);
 
 /* Embedding lookup with scaling, and the gradient of its table.
- *   (n / 64 * ceil(cols / 256) + vocab / 32 < 2^24.)
  *   fwd: out [n, cols] = scale * table[tokens[i], :]  (table [vocab, cols]).  A token outside the table sets err_flag (may be
- *        NULL) and reads row 0, as bf_embed_tokens does.
+ *        NULL) and reads row 0, as bf_embed_tokens does.  n * ceil(cols / 4) <= 2^31 - 4096 for an fp32 table, ceil(cols / 8)
+ *        for a 16-bit one; cols <= 2^30.
  *   bwd: grad [vocab, cols] fp32 = scale * the sum of the rows of dy [n, ld_dy] that share the token; accumulate != 0 adds to
  *        what is there instead and touches the rows of tokens that occur only.  Rows of the token padding_idx (-1: none) and
  *        of tokens outside the table (which set err_flag) are left out.  Sums are fp32, in a fixed order.
- *        workspace: bf_embed_scaled_bwd_workspace_bytes (0 for n <= 512), 16-byte aligned; n <= 2^30. */
+ *        workspace: bf_embed_scaled_bwd_workspace_bytes (0 for n <= 512), 16-byte aligned.  n <= 2^30, cols <= 2^30,
+ *        vocab < 2^31 - 1, and (in whole numbers) (n / 16 + 1) * S / 4 + vocab / 32 < 2^24 - 2 with S = ceil(cols / 256) for an
+ *        fp32 dy, ceil(cols / 512) for a 16-bit one. */
 int bf_embed_scaled_fwd(const int32_t* tokens, const void* table, int table_dtype, void* out, int out_dtype, float scale, int n,
                         int cols, int vocab, int* err_flag, bf_stream_t stream);
 size_t bf_embed_scaled_bwd_workspace_bytes(int n, int cols, int vocab);

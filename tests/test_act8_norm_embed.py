@@ -285,3 +285,38 @@ def test_overlap_against_the_addresses(L, seed):
             assert says == meet or (far and says)
         assert says or not meet, (a.shape, a.stride(), b.shape, b.stride())
     assert exact > 20
+
+
+def test_size_limits_as_the_header_states_them(L):
+    """One step over each limit is refused for its size; at the limit of the gradient the next check (a workspace of one byte)
+    is what refuses."""
+    lib = L.lib
+    most = 2 ** 31 - 4096
+    for dtype, v in ((L.F32, 4), (L.BF16, 8), (L.F16, 8)):
+        for cols in (1, v, v + 1, 1000, 1 << 30):
+            n = most // -(-cols // v) + 1
+            if n < 2 ** 31:
+                refused(L, lib.bf_embed_scaled_fwd(PTR, PTR, dtype, PTR, dtype, 1.0, n, cols, 100, None, None), -1, "too large")
+    refused(L, lib.bf_embed_scaled_fwd(PTR, PTR, L.F32, PTR, L.F32, 1.0, 1, (1 << 30) + 1, 100, None, None), -1, "bad shape")
+    refused(L, lib.bf_act8_pack(PTR, 33, L.F16, PTR, PTR, (2 ** 29 - 1024) // 2 + 1, 33, None), -1, "2^34")
+
+    def bwd(dt, n, cols, vocab):
+        return lib.bf_embed_scaled_bwd(PTR, cols, dt, PTR, PTR, 1.0, 0, -1, n, cols, vocab, None, PTR, 1, None)
+
+    def fits(n, cols, vocab, width):
+        return (n // 16 + 1) * -(-cols // width) // 4 + vocab // 32 < 2 ** 24 - 2
+
+    for dt, width in ((L.F32, 256), (L.BF16, 512), (L.F16, 512)):
+        for cols in (1, width, width + 1, 40 * width):
+            for vocab in (1, 2 ** 28, 2 ** 29 - 10 ** 6):
+                low, high = 513, 2 ** 30                            # the largest n that fits
+                if not fits(low, cols, vocab, width):
+                    continue
+                while low < high:
+                    mid = (low + high + 1) // 2
+                    low, high = (mid, high) if fits(mid, cols, vocab, width) else (low, mid - 1)
+                refused(L, bwd(dt, low, cols, vocab), -4, "workspace")
+                if low < 2 ** 30:
+                    refused(L, bwd(dt, low + 1, cols, vocab), -1, "too large")
+                else:
+                    refused(L, bwd(dt, low + 1, cols, vocab), -1, "2^30")

@@ -805,3 +805,22 @@ def test_outputs_in_columns_of_the_inputs_buffer(ops, L, gpu, cols, wide, dtype)
     y, _, _ = ops.rmsnorm_fwd(src, gamma, dtype, delta=delta, x_out=dst)
     assert torch.equal(y, want) and torch.equal(dst, total) and torch.equal(buf[:, :2 * cols], before[:, :2 * cols])
     assert torch.equal(buf[:, 3 * cols:], before[:, 3 * cols:])
+
+
+# ------------------------------------------------------------------ the lookup's longest form on odd widths
+@pytest.mark.parametrize("n,cols", [(17000, 1027), (2101, 8179)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embed_lookup_of_many_odd_rows(ops, gpu, n, cols, dtype):
+    """Over 2^21 vectors of 4 (fp32) or 8 elements and no whole number of 1 024: four vectors a lane, the last workgroup's
+    lanes past the end."""
+    many = n * -(-cols // (4 if dtype == torch.float32 else 8))
+    assert many >= 1 << 21 and many % 1024
+    g = torch.Generator(device="cuda").manual_seed(n)
+    table = torch.randn(777, cols, generator=g, device=gpu).to(dtype)
+    ids = torch.randint(0, 777, (n,), generator=g, device=gpu, dtype=torch.int32)
+    ids[n - 1] = 776
+    flag = torch.zeros(1, dtype=torch.int32, device=gpu)
+    for od in TYPES:
+        out = ops.embed_scaled_fwd(ids, table, 3.0, flag, od)
+        assert torch.equal(out, (table[ids.long()].float() * 3.0).to(od))
+    assert flag.item() == 0
