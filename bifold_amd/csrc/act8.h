@@ -4,10 +4,10 @@
 // A row is cut into groups of 32 columns, the last one possibly shorter.  A group shares one power of two, 2^e, with e the
 // smallest exponent for which round(max |x| 2^-e) <= 127 (and >= -126); element x is kept as q = round(x 2^-e), ties to
 // even, in int8, and reads back as q 2^e.  Powers of two make the scaling exact: the one rounding is q's, off by at most
-// 2^(e-1) <= max |x| / 127, and q 2^e is exact in fp32, bf16 and (inside its range) fp16.  A group of fp16 numbers whose largest
-// is 65 280 or more keeps it as 64 * 2^10, one step over fp16's range: unpacking to fp16 writes +-2^16 as +-65 504, so finite
-// fp16 values read back finite.  The byte kept per group is
-// code = e + 127, the exponent field of 2^e as a float: 1 .. 247.  A group that holds a NaN, an infinity or a magnitude of
+// 2^(e-1), which is at most max |x| / 127 (2^-127 where e = -126), and q 2^e is exact in fp32, bf16 and (inside its range)
+// fp16.  A group of fp16 numbers whose largest is 65 280 or more keeps it as 64 * 2^10, one step over fp16's range: unpacking
+// to fp16 writes +-2^16 as +-65 504, so finite fp16 values read back finite.  The byte kept per group is code = e + 127, the
+// exponent field of 2^e as a float: 1 .. 247.  A group that holds a NaN, an infinity or a magnitude of
 // 255 * 2^119 or more gets code 255, q = 0: 2^e is then infinity as a float and every element reads back as NaN, so an
 // overflow still reaches the gradients (a loss scaler's check sees it).
 #pragma once

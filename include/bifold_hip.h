@@ -654,7 +654,8 @@ int bf_gaussian_targets(const float* points, const int32_t* counts, float* heat,
  *   A row of x [rows, cols] (rows ld elements apart) is cut into groups of 32 columns, the last possibly shorter.  A group
  *   shares the power of two 2^e, e the smallest exponent >= -126 for which round(max |x| 2^-e) <= 127;
  *     q [rows, cols] int8 = round(x 2^-e), ties to even      code [rows, ceil(cols / 32)] uint8 = e + 127
- *   and x reads back as q 2^e: off by at most 2^(e-1) <= max |x| / 127.  A group with a NaN, an infinity or a magnitude of
+ *   and x reads back as q 2^e: off by at most 2^(e-1), which is at most max |x| / 127, or 2^-127 where e = -126 (a group
+ *   whose largest is 2^-127 or less reads back as zeros).  A group with a NaN, an infinity or a magnitude of
  *   255 * 2^119 or more has code 255 and reads back as NaN.  Unpacking to BF_F16 writes +-2^16, which fp16's numbers from
  *   65 280 on are kept as, as +-65 504 (larger values, from wider types, as infinities).
  * dtype: BF_F32 / BF_BF16 / BF_F16 of x, pre, y, dy, dpre.  rows * ceil(cols / 32) <= 2^29 - 1024.  Pointers need the alignment

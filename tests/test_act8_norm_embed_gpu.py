@@ -824,3 +824,24 @@ def test_embed_lookup_of_many_odd_rows(ops, gpu, n, cols, dtype):
         out = ops.embed_scaled_fwd(ids, table, 3.0, flag, od)
         assert torch.equal(out, (table[ids.long()].float() * 3.0).to(od))
     assert flag.item() == 0
+
+
+# ------------------------------------------------------------------ each group's own error
+@pytest.mark.parametrize("cols", [32, 70, 1024])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_act8_error_of_each_group(ops, gpu, cols, dtype):
+    """Rows of every magnitude: an element is off by half a step, which is at most its group's largest / 127, or 2^-127 where the
+    smallest step, 2^-126, is used."""
+    low, high = {torch.float32: (-149, 126), torch.bfloat16: (-133, 126), torch.float16: (-24, 14)}[dtype]
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(high - low + 1, cols, generator=g).clamp(-3, 3).double()
+    x = (x * torch.exp2(torch.arange(low, high + 1).double())[:, None] / 4).to(dtype)
+    q, code = ops.act8_pack(x.to(gpu))
+    back = ops.act8_unpack((q, code), torch.float32).cpu().double()
+    full = torch.zeros(2, x.shape[0], -(-cols // 32) * 32, dtype=torch.float64)
+    full[0, :, :cols], full[1, :, :cols] = x.double(), back
+    full = full.view(2, x.shape[0], -1, 32)
+    top = full[0].abs().amax(2)
+    half = torch.exp2(code.cpu().double() - 128)
+    assert ((full[0] - full[1]).abs() <= half[..., None]).all()
+    assert (half <= torch.maximum(top / 127, torch.full_like(top, 2.0 ** -127))).all()
