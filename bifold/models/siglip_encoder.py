@@ -347,7 +347,8 @@ class SiglipTowers(nn.Module):
                 # are re-made in the backward from x / xm -- one LayerNorm each and the fc1 GEMM, 30 % of a block's
                 # forward FLOPs; "full": only the block input x stays, the backward re-runs the block up to fc1
                 # (70 %).  The re-made tensors are bit for bit the forward's (same kernels, same inputs, the same
-                # dropout seeds), so gradients do not depend on the policy.  Measured at configs[2], B = 128, fp16
+                # dropout seeds), so gradients do not depend on the policy (with `lora_checkpoint: native`).  Measured at
+                # configs[2], B = 128, fp16
                 # (tools/lora_recompute_bench.py, five runs in one process each): none 198 samples/s at 181 GiB peak,
                 # mlp 190 at 147 GiB, full 179 at 109 GiB -- all stable since the dW side stream stopped pinning its
                 # operands with record_stream (pickplace._WeightGradSide).  Default: none (288 GB is there to be used).
@@ -358,8 +359,14 @@ class SiglipTowers(nn.Module):
                 # `lora_checkpoint: int8`: what is kept of the two stream tensors, of h1 and of the pre-activation is kept in
                 # 8 bits (ops.act8_pack: 33/32 bytes instead of 4 or 2 per element; every element within 1/127 of the largest
                 # of its 32 neighbours) -- none 26 -> 15.3, mlp 16 -> 10.1, full 4 -> 1.03 bytes x width per token and layer.
-                # The forward is untouched; the backward differentiates at the values that read back.  qkv and o keep their
-                # type: the backward takes exponentials of their products against the forward's log-sum-exp.  Measured
+                # The forward is untouched.  The backward takes the values that read back, with the forward's LayerNorm statistics
+                # (those of the unrounded stream) beside them where these are kept; what a policy re-makes from x or xm inherits
+                # their rounding, so gradients depend on the policy a little.  qkv and o keep their type: the backward takes
+                # exponentials of their products against the forward's log-sum-exp.  Distance of a tower's adapter gradients
+                # from native (tools/lora_checkpoint_error.py: full size, random weights, B = 8, fp16): vision 0.04 %, text 0.11 -
+                # 0.13 %, under every policy; with one column of the stream 30 larger 0.02 % and 0.4 - 0.8 %.  fp16 itself is
+                # 0.2 - 0.3 % from fp32 there.  q adapters whose gradient nearly cancels are fp16 noise either way (36 % from
+                # fp32); `full` moves them by another 57 %, `none` and `mlp` by 1 %.  Speed and memory
                 # (siglip_sequential, B = 128, fp16; samples/s and peak of the allocator, native -> int8): none 235.6 at
                 # 175.7 GiB -> 224.5 at 142.7; mlp 224.6 at 147.0 -> 220.2 at 129.6; full 210.6 at 111.5 -> 208.1 at 103.7.
                 if self.lora["checkpoint"] == "int8":

@@ -845,3 +845,72 @@ def test_act8_error_of_each_group(ops, gpu, cols, dtype):
     half = torch.exp2(code.cpu().double() - 128)
     assert ((full[0] - full[1]).abs() <= half[..., None]).all()
     assert (half <= torch.maximum(top / 127, torch.full_like(top, 2.0 ** -127))).all()
+
+
+# ------------------------------------------------------------------ how far the int8 gradients lie from the native ones
+# What a kept tensor's error does to an adapter's gradient: each use multiplies the gradient by a factor made of the tensor --
+# h1 in dY^T h1, x and xm through the normed rows of a LayerNorm's backward -- and moves it, relatively, by no more than the
+# tensor (a stream: than what is left of it without its mean); the GELU's slope by twice that (|act''| <= 1.13 against slopes
+# of some half).  Where tensors are made again from x or xm they inherit that error: `mlp` uses x twice (LayerNorm, h1) and xm
+# three times (LayerNorm, slope), `full` x eight times (LayerNorm, h1, q, k, v, xm, slope).  The roundings of different tensors
+# are independent, so the sum of all uses over all layers is an upper end of what they make together.
+USES = {"none": {"x": 1, "h1": 1, "xm": 1, "pre": 2}, "mlp": {"x": 2, "xm": 3}, "full": {"x": 8}}
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("outlier", [0.0, 30.0])
+@pytest.mark.parametrize("policy", ["none", "mlp", "full"])
+def test_int8_gradients_lie_near_the_native_ones(ops, gpu, dtype, outlier, policy):
+    """Relative distance of a tower's adapter gradients, int8 against native, under what the kept tensors' own errors allow; also
+    with one column of the residual stream far larger than the rest (its group's step is as coarse as that column)."""
+    from bifold.losses import Losses
+    from test_model_gpu import build_tiny_siglip
+    T, B = 2, 2
+    loss_fn = Losses.get_by_name(cfg=dict(name="bce_gaussmap", is_bimanual=True, mask_pick_heatmap=False))
+    g = torch.Generator().manual_seed(78)
+    sample = {"rgb": torch.randn(B, 3, 32, 32, generator=g), "rgb_context": torch.randn(B, T, 3, 32, 32, generator=g),
+              "instruction": torch.randint(0, 100, (B, 64), generator=g),
+              "context_attention_mask": torch.tensor([[1, 0], [1, 1]])}
+    for hn in ("left_pick", "left_place", "right_pick", "right_place"):
+        sample[f"{hn}_heatmap"] = torch.rand(B, 32, 32, generator=g)
+    sample = {k: v.to(gpu) for k, v in sample.items()}
+    grads, allowed = {}, {}
+    for how in ("native", "int8"):
+        torch.manual_seed(5)
+        model = build_tiny_siglip("siglip_sequential", True, dtype, gpu, T, lora=True, r=8, lora_dropout=0.0,
+                                  lora_recompute=policy, lora_checkpoint=how)
+        with torch.no_grad():
+            gb = torch.Generator().manual_seed(6)
+            for n, p in model.named_parameters():
+                if ".lora_B." in n:
+                    p.copy_(torch.randn(p.shape, generator=gb) * 0.05)
+                if n.endswith("position_embedding.weight"):
+                    p[:, 5] += outlier
+        model = model.to(gpu).train()
+        torch.manual_seed(9)
+        loss, _ = loss_fn(model(sample), sample)
+        if how == "native":
+            for tower, kept in model.siglip_model._saved.items():
+                total = 0.0
+                for S in kept["layers"]:
+                    for k, uses in USES[policy].items():
+                        t = S[k].double()
+                        off = ops.act8_unpack(ops.act8_pack(S[k]), torch.float32).double() - t
+                        size = t - t.mean(-1, keepdim=True) if k in ("x", "xm") else t
+                        total += uses * (off.norm() / size.norm()).item()
+                allowed[tower] = total
+        model.zero_grad()
+        loss.backward()
+        torch.cuda.synchronize()
+        for tower in allowed:
+            rows = [p.grad.detach().double().flatten() for n, p in model.named_parameters()
+                    if p.requires_grad and ".lora_" in n and tower in n]
+            assert len(rows) == 8
+            grads[how, tower] = torch.cat(rows)
+    for tower, most in allowed.items():
+        native, int8 = grads["native", tower], grads["int8", tower]
+        far = ((int8 - native).norm() / native.norm()).item()
+        cos = (torch.dot(int8, native) / (int8.norm() * native.norm())).item()
+        print(f"{tower} {policy} {dtype} outlier {outlier:g}: {far:.4f} of {most:.4f} allowed, cosine {cos:.6f}", flush=True)
+        assert 0 < far <= most and most < 1, (tower, far, most)
+        assert cos >= 1 - most * most / 2                        # what a relative distance of `most` allows, in first order
