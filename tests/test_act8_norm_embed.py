@@ -320,3 +320,35 @@ def test_size_limits_as_the_header_states_them(L):
                     refused(L, bwd(dt, low + 1, cols, vocab), -1, "too large")
                 else:
                     refused(L, bwd(dt, low + 1, cols, vocab), -1, "2^30")
+
+
+def test_polynomials_of_the_normal_tail():
+    """The coefficients in the source against Phi(-a) e^(a^2/2), in 64 bits: as near as the comments beside them say."""
+    import os
+    import re
+
+    import numpy as np
+    from scipy.special import erfcx
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "bifold_amd", "csrc", "act8.hip")).read()
+
+    def coefficients(name):
+        body = text[text.index(f"float {name}(float x, float& e) {{"):]
+        body = body[:body.index("return e * (r * q);")]
+        number = r"(-?[0-9.]+e[+-][0-9]+)f"
+        first = re.findall(r"float r = " + number, body)
+        return [np.float64(np.float32(c)) for c in first + re.findall(r"r = fmaf\(r, [uq], " + number, body)]
+
+    def horner(c, u):
+        r = np.zeros_like(u)
+        for v in c:
+            r = r * u + v
+        return r
+
+    for name, top, terms, near in (("normal_tail", 15.0, 9, 4.6e-8), ("normal_tail_fast", 14.3, 7, 7.95e-7)):
+        a = np.linspace(0, top, 300001)
+        c, q = coefficients(name), 1 / (a + 3.75)
+        assert len(c) == terms, name
+        got = q * horner(c, q if name.endswith("fast") else (a - 3.75) * q)
+        off = np.abs(got / (0.5 * erfcx(a / np.sqrt(2))) - 1).max()
+        assert off <= near, (name, off)
