@@ -345,7 +345,7 @@ def test_polynomials_of_the_normal_tail():
             r = r * u + v
         return r
 
-    for name, top, terms, near in (("normal_tail", 15.0, 9, 4.6e-8), ("normal_tail_fast", 14.3, 7, 7.95e-7)):
+    for name, top, terms, near in (("normal_tail", 15.0, 9, 4.6e-8), ("normal_tail_fast", 14.3, 7, 8.0e-7)):
         a = np.linspace(0, top, 300001)
         c, q = coefficients(name), 1 / (a + 3.75)
         assert len(c) == terms, name
