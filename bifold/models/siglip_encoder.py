@@ -365,7 +365,7 @@ class SiglipTowers(nn.Module):
                 # exponentials of their products against the forward's log-sum-exp.  Distance of a tower's adapter gradients
                 # from native (tools/lora_checkpoint_error.py: full size, random weights, B = 8, fp16): vision 0.04 %, text 0.11 -
                 # 0.13 %, under every policy; with one column of the stream 30 larger 0.02 % and 0.4 - 0.8 %.  fp16 itself is
-                # 0.2 - 0.3 % from fp32 there.  q adapters whose gradient nearly cancels are fp16 noise either way (36 % from
+                # 0.2 - 0.5 % from fp32 there.  q adapters whose gradient nearly cancels are fp16 noise either way (36 % from
                 # fp32); `full` moves them by another 57 %, `none` and `mlp` by 1 %.  Speed and memory
                 # (siglip_sequential, B = 128, fp16; samples/s and peak of the allocator, native -> int8): none 235.6 at
                 # 175.7 GiB -> 224.5 at 142.7; mlp 224.6 at 147.0 -> 220.2 at 129.6; full 210.6 at 111.5 -> 208.1 at 103.7.
