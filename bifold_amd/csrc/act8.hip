@@ -3,7 +3,8 @@
 //   bf_act8_unpack     q, code -> x
 //   bf_act8_gelu_fwd   pre -> y = act(pre), and the checkpoint of pre, in one pass
 //   bf_act8_gelu_bwd   dy, checkpoint -> dpre = dy act'(q 2^e)
-// All four stream: every byte is touched once and nothing is reused, so HBM bounds them and the layout is chosen for it.  A
+// All four stream: every byte is touched once and nothing is reused, so HBM bounds them (the 16-bit erf forward, at 4.8 TB/s,
+// its vector instructions) and the layout is chosen for it.  A
 // lane holds V = 8 consecutive elements (one 16-byte access of a 16-bit tensor, 8 bytes of q) or 4 of an fp32 tensor; a group
 // of 32 is a quad of lanes (or two), its maximum two (three) cross-lane moves without LDS.  One vector a lane and many
 // workgroups: 36 928 x 4 096 fp16 forward and backward 123 and 132 us, 6.2 and 5.8 TB/s (a copy of 2 GiB reaches 4.9, one of

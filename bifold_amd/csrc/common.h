@@ -154,7 +154,8 @@ __device__ __forceinline__ float erf_gelu_grad_f(float x) {
 // The accurate erff/expf above cost ~40 VALU instructions per element; in a GEMM epilogue
 // over 1.4e8 elements that is >150 us with the MFMA pipe idle.  16-bit outputs carry 2^-9 (bf16) / 2^-11 (fp16)
 // relative rounding, so the Abramowitz-Stegun 7.1.26 erf (|error| <= 1.5e-7: one v_exp, one
-// v_rcp, six FMAs) is three orders of magnitude below what the output can resolve.  The fp32
+// v_rcp, six FMAs) is three orders of magnitude below what the output can resolve next to values of order one; it is an
+// absolute error: the GELU's own small values at x < -4.5 lose digits and are 0 under -6 (act8.hip keeps them).  The fp32
 // ("exact") mode keeps the accurate functions.
 __device__ __forceinline__ float fast_erfc_abs(float az, float& e2) {   // erfc(|z|), e2 = exp(-z^2)
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, az, 1.0f));
